@@ -14,7 +14,8 @@ LIB_PATH = Path(__import__("os").environ.get("BSRL_LIB") or PKG / "_lib" / "libb
 HEADER = PKG.parent / "include" / "bsrl.h"
 
 N_ACT_HEADS = 29
-F32, F16, U8, I32, I64 = 0, 1, 2, 3, 4
+F32, F16, U8, I32, I64, BF16 = 0, 1, 2, 3, 4, 5
+INT8, E4M3 = 0, 1           # bsrl_kind8
 
 
 class BsrlError(RuntimeError):
@@ -144,6 +145,19 @@ _sig = {
                                  C.c_float, C.c_float, _P, _P, C.c_int64, _P, C.c_int64, _P]),
     "bsrl_linear_ln": (C.c_int, [_P, _P, _P, _P, _P, _P, C.c_float, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P]),
     "bsrl_qkv_attention_body": (C.c_int, [_P, _P, _P, _P, _P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, _P, _P]),
+    "bsrl_pack8_pitch": (C.c_int64, [C.c_int64]),
+    "bsrl_pack8": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _P, _P, _P]),
+    "bsrl_expand8": (C.c_int, [_P, _P, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P]),
+    "bsrl_gelu8": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int32, _P, _P, _P]),
+    "bsrl_gelu8_bwd": (C.c_int, [_P, C.c_int32, C.c_int64, _P, _P, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int64, _P]),
+    "bsrl_layernorm8": (C.c_int, [_P, _P, C.c_int32, C.c_int64, C.c_int64, _P, _P, C.c_float, C.c_int64, C.c_int32, _P, C.c_int64, _P,
+                                  C.c_int32, C.c_int64, C.c_int32, _P, _P, _P, _P, _P]),
+    "bsrl_layernorm8_bwd_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int32]),
+    "bsrl_layernorm8_bwd": (C.c_int, [_P, C.c_int32, C.c_int64, _P, C.c_int64, _P, _P, C.c_int32, _P, _P, _P, C.c_int64, C.c_int32, _P,
+                                      C.c_int32, C.c_int64, _P, _P, _P, C.c_int64, _P]),
+    "bsrl_linear8_wgrad_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    "bsrl_linear8_wgrad": (C.c_int, [_P, C.c_int32, C.c_int64, _P, _P, C.c_int32, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, C.c_int64,
+                                     _P]),
     "bsrl_attention_tokens": (C.c_int, [_P, _P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P]),
 }
 for _name, (_res, _args) in _sig.items():

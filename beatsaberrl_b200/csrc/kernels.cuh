@@ -371,4 +371,45 @@ int multi_pack(const bsrl_config& cfg, const Layout& l, float* const* params, co
                float beta2, float eps, int step, const float* inv_scale, const float* found_inf, void* arena,
                cudaStream_t stream);
 
+// Activations in 8 bits (pack8.cuh): codes (rows, pitch) with the pitch d rounded up to whole blocks of 32, exps (rows, pitch / 32).
+// Rows of elements have a pitch of their own; any alignment of theirs is served, 16 bytes faster.
+int pack8(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t d, int kind, uint8_t* codes, uint8_t* exps, cudaStream_t stream);
+int expand8(const uint8_t* codes, const uint8_t* exps, int kind, int64_t rows, int64_t d, void* out, int dtype, int64_t ldo, cudaStream_t stream);
+int gelu8(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t d, void* y, int64_t ldy, int kind, uint8_t* codes, uint8_t* exps,
+          cudaStream_t stream);
+int gelu8_bwd(const void* gy, int dtype, int64_t ldgy, const uint8_t* codes, const uint8_t* exps, int kind, int64_t rows, int64_t d, void* gx,
+              int64_t ldgx, cudaStream_t stream);
+// LayerNorm with its input kept in 8 bits (norm8.cuh)
+struct Norm8Args {
+  const void *x, *residual;      // residual: may be nullptr
+  void *z, *y;                   // z: with a residual only
+  const float *gamma, *beta;     // beta: may be nullptr
+  uint8_t *codes, *exps;
+  float *mean, *rstd;
+  int64_t rows, ldx, ldr, ldz, ldy;
+  int d, kind, dtype, y_dtype;
+  float eps;
+};
+struct Norm8BwdArgs {
+  const void *gy, *g_residual;   // g_residual: may be nullptr
+  void* gx;
+  const float* gamma;
+  const uint8_t *codes, *exps;
+  const float *mean, *rstd;
+  float *g_gamma, *g_beta;       // either may be nullptr
+  int64_t rows, ldgy, ldgr, ldgx;
+  int d, kind, dtype, gy_dtype;
+};
+bool norm8_types_ok(int dtype, int y_dtype);
+int norm8_max_width();
+int norm8_fwd(const Norm8Args& a, cudaStream_t stream);
+int64_t norm8_bwd_workspace(int64_t rows, int d);
+int norm8_bwd(const Norm8BwdArgs& a, float* workspace, cudaStream_t stream);
+
+// Weight and bias gradient of a linear layer from its input in 8 bits (wgrad8_tc5.cu); gb may be nullptr.  aligned: g and its pitch
+// are multiples of 16 bytes.
+int64_t wgrad8_workspace(int64_t rows, int n, int k, bool aligned);
+int wgrad8(const void* g, int g_dtype, int64_t ldg, const uint8_t* codes, const uint8_t* exps, int kind, int64_t rows, int n, int k, float* gw,
+           int64_t ldw, float* gb, void* workspace, int64_t workspace_bytes, cudaStream_t stream);
+
 }  // namespace bsrl

@@ -1,0 +1,19 @@
+// LayerNorm with its input kept in 8 bits: fp32 rows (norm8.cuh).
+#include "norm8.cuh"
+
+namespace bsrl {
+namespace norm8 {
+template <>
+int fwd(const FwdArgs<float, float>& p, bool vec, cudaStream_t stream) { return launch_fwd(p, vec, stream); }
+template <>
+int fwd(const FwdArgs<float, __half>& p, bool vec, cudaStream_t stream) { return launch_fwd(p, vec, stream); }
+template <>
+int fwd(const FwdArgs<float, __nv_bfloat16>& p, bool vec, cudaStream_t stream) { return launch_fwd(p, vec, stream); }
+template <>
+int bwd(const BwdArgs<float, float>& p, bool vec, cudaStream_t stream) { return launch_bwd(p, vec, stream); }
+template <>
+int bwd(const BwdArgs<float, __half>& p, bool vec, cudaStream_t stream) { return launch_bwd(p, vec, stream); }
+template <>
+int bwd(const BwdArgs<float, __nv_bfloat16>& p, bool vec, cudaStream_t stream) { return launch_bwd(p, vec, stream); }
+}  // namespace norm8
+}  // namespace bsrl

@@ -49,7 +49,7 @@ typedef enum bsrl_status {
 } bsrl_status;
 
 typedef enum bsrl_dtype {
-  BSRL_F32 = 0, BSRL_F16 = 1, BSRL_U8 = 2, BSRL_I32 = 3, BSRL_I64 = 4
+  BSRL_F32 = 0, BSRL_F16 = 1, BSRL_U8 = 2, BSRL_I32 = 3, BSRL_I64 = 4, BSRL_BF16 = 5
 } bsrl_dtype;
 
 /* Shape of the network: the keyword arguments of the reference constructor that change
@@ -277,6 +277,68 @@ int64_t bsrl_linear_bwd_scratch_bytes(int64_t m, int32_t n, int32_t k);
 int bsrl_linear_bwd(const void* g_f16, const void* x_f16, const void* w_f16, int64_t m, int32_t n, int32_t k,
                     float* g_weight, float* g_bias, void* g_x, int32_t g_x_f32, void* scratch, int64_t scratch_bytes,
                     void* stream);
+
+/* --- activations kept in 8 bits ------------------------------------------------------- *
+ * Operators of a training step that keep what their backward needs in 8 bits instead of 16 or 32: a minibatch's
+ * saved activations shrink to 33/64 (of 16-bit ones) or 33/128.
+ *
+ * A checkpoint of a (rows, d) matrix is two arrays without gaps: codes (rows, bsrl_pack8_pitch(d)) u8, 16-byte
+ * aligned, and exps (rows, bsrl_pack8_pitch(d) / 32) u8.  Blocks of 32 neighbouring values of a row (the last one of a row may be
+ * shorter; its codes end in zeros) share an exponent: value = code 2^(exp - 127), the code being
+ *   BSRL_INT8  an int8 in [-127, 127]:          off by at most 1/127 of the block's largest magnitude,
+ *   BSRL_E4M3  an e4m3 number in [-240, 240]:   off by at most 2^-4 of the value itself, or 2^-16 of the block's largest.
+ * exp is the least one with which the code of the largest magnitude, rounded to nearest (ties to even), is in that range.  In the
+ * top binade of the matrix's type it does not grow further and codes clamp: every value is finite in that type.  exp = 0: zeros
+ * (largest magnitude below 2^-120, E4M3 2^-119).  A block with an infinity or NaN stands for 32 NaN (exp 255, codes 0).
+ * Values have at most 8 significant bits: bf16 holds them exactly, fp16 as far as its range goes.
+ *
+ * Matrices have elements of BSRL_F32, BSRL_F16 or BSRL_BF16, rows `ld` elements apart (ld >= d) and no alignment but
+ * their elements'; rows that start on 16 bytes, with d a multiple of 8, are faster.  rows may be 0.  d up to 2^31 - 64
+ * (bsrl_layernorm8: 16,384).  gamma, beta, mean, rstd and parameter gradients are fp32.  Sums are in fp32 and in one
+ * order: a call on the same inputs gives the same bits.  Nothing may overlap except where said. */
+typedef enum bsrl_kind8 { BSRL_INT8 = 0, BSRL_E4M3 = 1 } bsrl_kind8;
+
+int64_t bsrl_pack8_pitch(int64_t d);     /* d rounded up to a multiple of 32 (-1: d out of range) */
+int bsrl_pack8(const void* x, int32_t dtype, int64_t ldx, int64_t rows, int64_t d, int32_t kind, uint8_t* codes,
+               uint8_t* exps, void* stream);
+/* out = what the checkpoint stands for, rounded to `dtype` */
+int bsrl_expand8(const uint8_t* codes, const uint8_t* exps, int32_t kind, int64_t rows, int64_t d, void* out,
+                 int32_t dtype, int64_t ldo, void* stream);
+
+/* Exact (erf) GELU whose input is kept in 8 bits: y = gelu(x) (y may be x), codes / exps = checkpoint of x.
+ * bsrl_gelu8_bwd: gx = gy gelu'(x8) (gx may be gy); gy and gx have the same type. */
+int bsrl_gelu8(const void* x, int32_t dtype, int64_t ldx, int64_t rows, int64_t d, void* y, int64_t ldy, int32_t kind,
+               uint8_t* codes, uint8_t* exps, void* stream);
+int bsrl_gelu8_bwd(const void* gy, int32_t dtype, int64_t ldgy, const uint8_t* codes, const uint8_t* exps, int32_t kind,
+                   int64_t rows, int64_t d, void* gx, int64_t ldgx, void* stream);
+
+/* LayerNorm whose input is kept in 8 bits, with the residual sum in front of it:
+ *   z = x + residual rounded to `dtype` (residual NULL: z = x, and the z argument is not used; z may be x or residual)
+ *   y = (z - mean) rstd gamma + beta in y_dtype;  codes / exps = checkpoint of z;  mean, rstd (rows) of z itself
+ * beta may be NULL (none).  Rows of BSRL_F32 give y in any of the three types, 16-bit rows y in their own.
+ * bsrl_layernorm8_bwd, with h = (z8 - mean) rstd and gh = gy gamma:
+ *   gx = rstd (gh - mean(gh) - h mean(gh h)) (+ g_residual, the gradient that reaches z by other ways; may be NULL), in `dtype`
+ *   g_gamma = sum over rows of gy h, g_beta = sum over rows of gy (written, not added to; either may be NULL)
+ * gx is the gradient of x and of the residual.  gx may be g_residual, or gy where the types agree.  workspace:
+ * bsrl_layernorm8_bwd_workspace_bytes() of device memory, 16-byte aligned (0 bytes: may be NULL). */
+int bsrl_layernorm8(const void* x, const void* residual, int32_t dtype, int64_t ldx, int64_t ldr, const float* gamma,
+                    const float* beta, float eps, int64_t rows, int32_t d, void* z, int64_t ldz, void* y, int32_t y_dtype,
+                    int64_t ldy, int32_t kind, uint8_t* codes, uint8_t* exps, float* mean, float* rstd, void* stream);
+int64_t bsrl_layernorm8_bwd_workspace_bytes(int64_t rows, int32_t d);
+int bsrl_layernorm8_bwd(const void* gy, int32_t gy_dtype, int64_t ldgy, const void* g_residual, int64_t ldgr,
+                        const uint8_t* codes, const uint8_t* exps, int32_t kind, const float* mean, const float* rstd,
+                        const float* gamma, int64_t rows, int32_t d, void* gx, int32_t dtype, int64_t ldgx, float* g_gamma,
+                        float* g_beta, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Weight and bias gradient of y = x w^T + b from x (rows, k) kept in 8 bits and gy (rows, n) f16 or bf16, on the tcgen05 tensor
+ * cores: g_weight (n, k) = gy^T x8, g_bias (n) = column sums of gy (NULL: none); written, not added to.  x8 enters the product in
+ * gy's type.  rows up to 2^31 - 257, n and k up to 2^20.  workspace: bsrl_linear8_wgrad_workspace_bytes() of device
+ * memory, 256-byte aligned; `aligned` says that gy starts on 16 bytes and ldgy is a multiple of 8 (else the workspace also takes
+ * a copy of gy that is). */
+int64_t bsrl_linear8_wgrad_workspace_bytes(int64_t rows, int32_t n, int32_t k, int32_t aligned);
+int bsrl_linear8_wgrad(const void* gy, int32_t gy_dtype, int64_t ldgy, const uint8_t* codes, const uint8_t* exps,
+                       int32_t kind, int64_t rows, int32_t n, int32_t k, float* g_weight, float* g_bias, void* workspace,
+                       int64_t workspace_bytes, void* stream);
 
 /* --- the single-body-token layout ---------------------------------------------------- *
  * A second front / back end around the same transformer core, for policies laid out as one body token
