@@ -1,16 +1,23 @@
 // Weight gradient of a linear layer from an input that was kept in 8 bits (pack8.cuh):
 //   g_weight (n, k) = g^T x8,  g_bias (n) = column sums of g,  over `rows` rows; g 16-bit, results fp32.
 //
-// Persistent, warp-specialised tcgen05 kernel.  The contraction runs over rows, so both operands are MN-major tiles of 64 rows as they
-// lie in memory:
-//   warp 0       TMA producer: (64 rows x 128 MH columns) of g per stage, 128-byte swizzle, columns and rows past the ends as zeros;
-//   warp 1       MMA issuer: per stage MH accumulators of 128 x BN in TMEM (MH = 2, BN = 256: all of it), the x tile read by both;
-//   warps 2..9   converters: 16 codes per 16-byte load, requested a stage ahead, to the 16-bit type of g (exact: the scale is a power of
-//                two) and into the swizzled tile; after a chain they drain the accumulators;
-//   warps 10..13 column sums of g from the stage, for the first column tile's work items only (no second read of g).
+// Persistent, warp-specialised tcgen05 kernel, one CTA per SM or (CTAS = 2) pairs of CTAs on neighbouring SMs.  The contraction runs
+// over rows, so both operands are MN-major tiles of 64 rows as they lie in memory; a tile of the result has 128 CTAS x BN elements:
+//   warp 0        TMA producer of g: 64 rows x the CTA's own 128 columns per stage, columns and rows past the ends as zeros;
+//   warp 1        MMA issuer (a pair's leader's), into one of two accumulators of BN columns in TMEM;
+//   warps 2..17   converters: 16 codes per 16-byte load to the 16-bit type of g (exact: the scale is a power of two), into the swizzled
+//                 tile that the MMAs (of both CTAs) read.  Groups of warps take stages in turn and request a stage's codes before they wait for its
+//                 slot, so several stages' loads are under way;
+//   warps 18..21  drain: accumulators to the workspace while the next chain runs into the other accumulator;
+//   warps 22..25  column sums of g from the stage, for the first column tile's work items only (no second read of g).
+// Why groups: the proxy fence ahead of a converter's arrival waits for all loads its thread has in flight, so a thread cannot hold the
+// next stages' codes in registers (that took 2,150 cycles a stage, a load's latency each).  Codes through a TMA ring instead cost the shared
+// memory 16 KB a stage, which is what bounds the kernel together with the issue slots: 1,310 cycles a stage with column sums, 1,030 without.
 // A work item is (tile, piece of the rows).  The pieces' partial tiles go to the workspace and a second kernel adds them in order: the
 // same bits every time.  Inside an item the accumulators are drained every kChain stages and added in fp32, rounded to nearest: the tensor
-// core's own running sum truncates, about 2e-8 of the sum per 16 rows (475,136 rows in one chain per CTA were 7.6e-6 off).
+// core's own running sum truncates, about 2e-8 of the sum per 16 rows (475,136 rows in chains of 6,420 were 7.6e-6 off, of 2,048 2e-6).
+// A pair halves what a CTA converts and what its MMAs read of shared memory: with one CTA and two accumulators of 256 columns beside each
+// other (no second set to drain from) the shared memory's 128 bytes per cycle bound the stage, and every drain stopped the MMAs.
 // All waits are bounded (tc5.cuh); a wait that runs out sets the device status word and every role falls through to the teardown.
 #include <cmath>
 
@@ -26,21 +33,30 @@ using namespace p8;
 constexpr int KERNEL_ID = 14;
 constexpr int BK = 64;                           // rows per stage
 constexpr int BLOCK_BYTES = BK * 128;            // 64 columns x 64 rows of 16 bits
-constexpr int CONV_WARPS = 8, SUM_WARPS = 4;
-constexpr int THREADS = (2 + CONV_WARPS + SUM_WARPS) * 32;
+constexpr int G_BYTES = 2 * BLOCK_BYTES;         // 128 columns of g
+constexpr int CONV_WARPS = 16, DRAIN_WARPS = 4, SUM_WARPS = 4;
+constexpr int groups_of(int ctas) { return ctas == 2 ? 4 : 2; }                // of converters, which take stages in turn
+constexpr int sum_groups(int ctas) { return ctas == 2 ? 4 : 2; }               // of sum warps, likewise
+constexpr int CONV0 = 2, DRAIN0 = CONV0 + CONV_WARPS, SUM0 = DRAIN0 + DRAIN_WARPS;      // first warp of each role
+constexpr int THREADS = (SUM0 + SUM_WARPS) * 32;
 constexpr int MAX_BN = 256;
-constexpr int TMEM_COLS = 512;
-constexpr int kChain = 64;                       // stages between drains: 4,096 rows
-constexpr int stages_of(int mh) { return mh == 2 ? 3 : 4; }
-constexpr int stage_bytes(int mh) { return (2 * mh + 4) * BLOCK_BYTES; }
-constexpr int smem_bytes(int mh) { return stages_of(mh) * stage_bytes(mh) + 1024 /*alignment*/ + 256 /*barriers*/; }
-constexpr int phases_of(int mh) { return SUM_WARPS * 32 / (16 * mh); }      // threads that share eight columns of g
+constexpr int TMEM_COLS = 2 * MAX_BN;
+constexpr int kChain = 32;                       // stages between drains: 2,048 rows
+constexpr int PHASES = SUM_WARPS * 32 / 16;      // threads that share eight columns of g
+constexpr int stages_of(int ctas) { return ctas == 2 ? 6 : 4; }
+constexpr int stage_bytes(int ctas) { return G_BYTES + 4 / ctas * BLOCK_BYTES; }
+constexpr int smem_bytes(int ctas) { return stages_of(ctas) * stage_bytes(ctas) + 1024 /*alignment*/ + 512 /*barriers*/; }
+// A group that has seen stage i - groups knows that the slot of stage i has been through stage i - stages_of: without that its wait could
+// take the phase before the last one for the last one
+static_assert(groups_of(1) <= stages_of(1) && groups_of(2) <= stages_of(2) && sum_groups(1) <= stages_of(1) && sum_groups(2) <= stages_of(2), "phases");
+static_assert(smem_bytes(1) <= 227 * 1024 && smem_bytes(2) <= 227 * 1024, "shared memory");
 
 struct Shared {
-  uint64_t full_g[4], full_x[4], empty[4], acc_full, acc_empty, mma_done;
+  uint64_t full_g[6], full_x[6], empty[6], acc_full[2], acc_empty[2], mma_done;
   uint32_t tmem_base;
   int abort;
 };
+static_assert(sizeof(Shared) <= 512, "barrier space");
 __device__ __forceinline__ void give_up(Shared* sh, int* status, int role) {
   atomicCAS(status, 0, KERNEL_ID * 16 + role);
   sh->abort = 1;
@@ -51,272 +67,356 @@ struct Args {
   const uint8_t* exps;
   int64_t rows;
   int64_t pitch;                 // of the codes
-  int n, bn;                     // bn: columns of a tile of x
-  int k_tiles, tiles, splits;    // tiles = n tiles x k tiles
+  int bn;                        // columns of a tile of x
+  int n_tiles, k_tiles, splits;
   int k_blocks;                  // stages of all rows
-  float* parts;                  // (tiles, splits, 4 MH, bn, 32)
-  float* bias_parts;             // (splits, phases, n tiles x 128 MH), nullptr: no column sums
+  float* parts;                  // (tiles, splits, 4 CTAS, bn / 4, 32 rows, 4 columns)
+  float* bias_parts;             // (splits, PHASES, n_tiles x 128 CTAS), nullptr: no column sums
 };
 
-// Item w -> (tile, split): the splits of a tile are neighbours, the k tiles of the same rows run at the same time
+// Item w -> (split, n tile, k tile), split-major: the tiles of the same rows run at the same time
 struct Item {
-  int tile, split, nt, kt, kb0, kb1;
+  int split, nt, kt, kb0, kb1;
 };
 __device__ __forceinline__ Item item_of(int w, const Args& p) {
   Item it;
-  it.split = w / p.tiles;
-  it.tile = w - it.split * p.tiles;
-  it.nt = it.tile / p.k_tiles;
-  it.kt = it.tile - it.nt * p.k_tiles;
+  const int tiles = p.n_tiles * p.k_tiles;
+  it.split = w / tiles;
+  const int tile = w - it.split * tiles;
+  it.nt = tile / p.k_tiles;
+  it.kt = tile - it.nt * p.k_tiles;
   it.kb0 = (int)((int64_t)p.k_blocks * it.split / p.splits);
   it.kb1 = (int)((int64_t)p.k_blocks * (it.split + 1) / p.splits);
   return it;
 }
 
-template <typename TG, int KIND, int MH>
+// a, b += the two 16-bit numbers of w, in fp32
+template <typename TG>
+__device__ __forceinline__ void add_pair(uint32_t w, float& a, float& b) {
+  if (top_binade<TG>() == 15)
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.f32.f16 %0, l, %0;\n\tadd.f32.f16 %1, h, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(w));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.f32.bf16 %0, l, %0;\n\tadd.f32.bf16 %1, h, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(w));
+}
+
+// 16 codes and their exponent -> 16 numbers of 16 bits, two at a time where the scale allows it
+template <typename TG, int KIND>
+__device__ __forceinline__ void convert16(const uint4& code, uint32_t e, uint32_t (&o)[8]) {
+  const uint32_t w[4] = {code.x, code.y, code.z, code.w};
+  constexpr bool F16 = top_binade<TG>() == 15;
+  if (F16 && e - 113u < 19u) {               // 2^-14 .. 2^4: the scale, and 1152 times it, are normal fp16 numbers
+    const uint32_t sc = ((e - 112u) << 10) * 0x10001u;
+    const __half2 s2 = *reinterpret_cast<const __half2*>(&sc);
+    const __half2 off = __hmul2(s2, __floats2half2_rn(-1152.f, -1152.f));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t lo, hi;
+      __half2 a, b;
+      if (KIND == kInt8) {
+        const uint32_t u = w[j] ^ 0x80808080u;                                // 1152 + code = 1024 + (code + 128)
+        lo = __byte_perm(u, 0x64646464u, 0x4140);
+        hi = __byte_perm(u, 0x64646464u, 0x4342);
+        a = __hfma2(*reinterpret_cast<__half2*>(&lo), s2, off);               // code x scale, exactly
+        b = __hfma2(*reinterpret_cast<__half2*>(&hi), s2, off);
+      } else {
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w[j]));
+        a = __hmul2(*reinterpret_cast<__half2*>(&lo), s2);
+        b = __hmul2(*reinterpret_cast<__half2*>(&hi), s2);
+      }
+      o[2 * j] = *reinterpret_cast<uint32_t*>(&a);
+      o[2 * j + 1] = *reinterpret_cast<uint32_t*>(&b);
+    }
+    return;
+  }
+  const float s = scale_of(e);
+  if (!F16 && KIND == kInt8 && e - 1u < 200u) {           // 2^23 times the scale is finite
+    const uint64_t s2 = f2_make(s, s), off = f2_make(-8388736.f * s, -8388736.f * s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t u = w[j] ^ 0x80808080u;
+      float a, b, c, d;
+      f2_split(f2_fma(f2_make(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7651))), s2, off), a, b);
+      f2_split(f2_fma(f2_make(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7652)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7653))), s2, off), c, d);
+      o[2 * j] = pack2<TG>(a, b);
+      o[2 * j + 1] = pack2<TG>(c, d);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float a, b, c, d;
+    decode4<KIND>(w[j], a, b, c, d);
+    o[2 * j] = pack2<TG>(a * s, b * s);
+    o[2 * j + 1] = pack2<TG>(c * s, d * s);
+  }
+}
+
+template <typename TG, int KIND, int CTAS>
 __global__ void __launch_bounds__(THREADS, 1)
 wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
-  constexpr int STAGES = stages_of(MH), STAGE_BYTES = stage_bytes(MH), G_BYTES = 2 * MH * BLOCK_BYTES;
+  constexpr bool PAIR = CTAS == 2;
+  constexpr int STAGES = stages_of(CTAS), STAGE_BYTES = stage_bytes(CTAS);
+  constexpr int GROUPS = groups_of(CTAS), GROUP_WARPS = CONV_WARPS / GROUPS;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* tiles_ptr = smem_raw + (base - raw);
   Shared* sh = reinterpret_cast<Shared*>(tiles_ptr + STAGES * STAGE_BYTES);
+  const int own = p.bn / CTAS;                // columns of the x tile that this CTA converts
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = PAIR ? (int)cluster_rank() : 0;
   volatile int* abort = &sh->abort;
-  const int n_items = p.tiles * p.splits;
+  const int n_items = p.n_tiles * p.k_tiles * p.splits;
+  const int w_first = (int)blockIdx.x / CTAS, w_step = (int)gridDim.x / CTAS;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&sh->full_g[s]), 1);
-      mbar_init(smem_u32(&sh->full_x[s]), CONV_WARPS);
-      mbar_init(smem_u32(&sh->empty[s]), 1 + (p.bias_parts ? SUM_WARPS : 0));
+      mbar_init(smem_u32(&sh->full_x[s]), CTAS * GROUP_WARPS);       // the leader's: both CTAs' converters
+      mbar_init(smem_u32(&sh->empty[s]), 1 + (p.bias_parts ? SUM_WARPS / sum_groups(CTAS) : 0));
     }
-    mbar_init(smem_u32(&sh->acc_full), 1);
-    mbar_init(smem_u32(&sh->acc_empty), CONV_WARPS);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&sh->acc_full[b]), 1);
+      mbar_init(smem_u32(&sh->acc_empty[b]), CTAS * DRAIN_WARPS);   // the leader's: both CTAs' drain warps
+    }
     mbar_init(smem_u32(&sh->mma_done), 1);
     sh->abort = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_g);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(&sh->tmem_base), TMEM_COLS);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(smem_u32(&sh->tmem_base), TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(&sh->tmem_base), TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();          // the peer's barriers exist before anything is signalled across
   tc_fence_after();
   const uint32_t tmem_base = sh->tmem_base;
   pdl_begin();
+  // an arrival at the leader's barrier
+  auto arrive_leader = [&](uint64_t* bar) {
+    if (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(bar), 0));
+    else mbar_arrive(smem_u32(bar));
+  };
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     if (lane == 0) {
-      uint32_t it = 0;
+      uint32_t it = 0, s = 0, phase = 0;
       bool ok = true;
-      for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
+      for (int w = w_first; w < n_items && ok; w += w_step) {
         const Item m = item_of(w, p);
+        const int x = (m.nt * CTAS + rank) * 128;
         for (int kb = m.kb0; kb < m.kb1; ++kb, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait(smem_u32(&sh->empty[s]), ((it / STAGES) & 1) ^ 1, abort)) { give_up(sh, status, 1); ok = false; break; }
-          const uint32_t bar = smem_u32(&sh->full_g[s]);
+          if (!mbar_wait(smem_u32(&sh->empty[s]), phase ^ 1, abort)) { give_up(sh, status, 1); ok = false; break; }
+          const uint32_t bar = smem_u32(&sh->full_g[s]), dst = base + s * STAGE_BYTES;
           mbar_expect_tx(bar, G_BYTES);
-#pragma unroll
-          for (int b = 0; b < 2 * MH; ++b) tma_load_2d(base + s * STAGE_BYTES + b * BLOCK_BYTES, &tm_g, m.nt * (128 * MH) + b * 64, kb * BK, bar);
+          tma_load_2d(dst, &tm_g, x, kb * BK, bar);
+          tma_load_2d(dst + BLOCK_BYTES, &tm_g, x + 64, kb * BK, bar);
+          if (++s == STAGES) { s = 0; phase ^= 1; }
         }
       }
       // what is in flight must land before this CTA may exit (bounded, ignoring abort)
-      for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j) {
-        uint32_t spins = 0;
+      uint32_t spins = 0;
+      for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
         while (!mbar_try_wait(smem_u32(&sh->full_g[j % STAGES]), (j / STAGES) & 1) && ++spins < kSpinLimit) {}
-        if (spins >= kSpinLimit) give_up(sh, status, 2);
-      }
+      if (spins >= kSpinLimit) give_up(sh, status, 2);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      uint32_t it = 0, chains = 0;
+    if (lane == 0 && rank == 0) {
+      // One thread issues everything: slots, phases and descriptors by counters, nothing derived per stage
+      uint32_t slot = 0, phase = 0, buf = 0, acc_phase = 1;
       bool ok = true;
-      uint32_t idesc = idesc_f16(128, p.bn, 1, 1);
-      if (sizeof(TG) == 2 && top_binade<TG>() == 127) idesc |= (1u << 7) | (1u << 10);      // both operands bf16
-      for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
+      uint32_t idesc = idesc_f16(128 * CTAS, p.bn, 1, 1);
+      if (top_binade<TG>() == 127) idesc |= (1u << 7) | (1u << 10);      // both operands bf16
+      const uint64_t g0 = smem_desc_mn_sw128(base, BLOCK_BYTES), x0 = smem_desc_mn_sw128(base + G_BYTES, BLOCK_BYTES);
+      for (int w = w_first; w < n_items && ok; w += w_step) {
         const Item m = item_of(w, p);
-        for (int kb = m.kb0; kb < m.kb1; ++kb, ++it) {
-          const int pos = (kb - m.kb0) % kChain;
-          if (pos == 0) {
-            if (!mbar_wait(smem_u32(&sh->acc_empty), (chains & 1) ^ 1, abort)) { give_up(sh, status, 3); ok = false; break; }
-            ++chains;
-          }
-          const int s = it % STAGES;
-          const uint32_t ph = (it / STAGES) & 1;
-          if (!mbar_wait(smem_u32(&sh->full_g[s]), ph, abort) || !mbar_wait(smem_u32(&sh->full_x[s]), ph, abort)) { give_up(sh, status, 4); ok = false; break; }
+        for (int left = m.kb1 - m.kb0; left > 0 && ok; left -= kChain) {
+          if (!mbar_wait<PAIR>(smem_u32(&sh->acc_empty[buf]), acc_phase, abort)) { give_up(sh, status, 3); ok = false; break; }
           tc_fence_after();
-          const uint32_t g_addr = base + s * STAGE_BYTES;
-          const uint64_t x_desc = smem_desc_mn_sw128(g_addr + G_BYTES, BLOCK_BYTES);
+          const uint32_t d = tmem_base + buf * MAX_BN;
+          const int n = min(left, kChain);
+          for (int i = 0; i < n; ++i) {
+            // the converters' arrivals stand for g too
+            if (!mbar_wait<PAIR>(smem_u32(&sh->full_x[slot]), phase, abort)) { give_up(sh, status, 4); ok = false; break; }
+            tc_fence_after();
+            const uint64_t g_desc = g0 + slot * (STAGE_BYTES >> 4), x_desc = x0 + slot * (STAGE_BYTES >> 4);
 #pragma unroll
-          for (int h = 0; h < MH; ++h) {
-            const uint64_t g_desc = smem_desc_mn_sw128(g_addr + h * 2 * BLOCK_BYTES, BLOCK_BYTES);
-#pragma unroll
-            for (int k = 0; k < BK / 16; ++k) mma_f16_ss(tmem_base + h * MAX_BN, g_desc + 128 * k, x_desc + 128 * k, idesc, (pos || k) ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) {
+              if (PAIR) mma_f16_ss_pair(d, g_desc + 128 * k, x_desc + 128 * k, idesc, (i || k) ? 1u : 0u);
+              else mma_f16_ss(d, g_desc + 128 * k, x_desc + 128 * k, idesc, (i || k) ? 1u : 0u);
+            }
+            PAIR ? tc_commit_pair(smem_u32(&sh->empty[slot])) : tc_commit(smem_u32(&sh->empty[slot]));
+            if (++slot == STAGES) { slot = 0; phase ^= 1; }
           }
-          tc_commit(smem_u32(&sh->empty[s]));
-          if (pos == kChain - 1 || kb == m.kb1 - 1) tc_commit(smem_u32(&sh->acc_full));
+          if (ok) PAIR ? tc_commit_pair(smem_u32(&sh->acc_full[buf])) : tc_commit(smem_u32(&sh->acc_full[buf]));
+          acc_phase ^= buf;
+          buf ^= 1;
         }
       }
       // every MMA issued must have retired before TMEM is freed (bounded, ignoring abort)
-      tc_commit(smem_u32(&sh->mma_done));
+      PAIR ? tc_commit_pair(smem_u32(&sh->mma_done)) : tc_commit(smem_u32(&sh->mma_done));
       uint32_t spins = 0;
       while (!mbar_try_wait(smem_u32(&sh->mma_done), 0) && ++spins < kSpinLimit) {}
       if (spins >= kSpinLimit) give_up(sh, status, 5);
     }
-  } else if (warp < 2 + CONV_WARPS) {
-    // ---------------------------------------------------------------- converters, then the drain
-    const int t = threadIdx.x - 64;                // 0 .. 255
-    const int per_row = p.bn / 16, n_pieces = per_row * BK;
-    constexpr int MAX_P = MAX_BN / 16 * BK / (CONV_WARPS * 32);       // pieces of 16 codes per thread and stage: 4
-    int row[MAX_P], piece[MAX_P];
-    uint32_t dst[MAX_P];
-#pragma unroll
-    for (int i = 0; i < MAX_P; ++i) {
-      const int q = t + i * CONV_WARPS * 32;
-      row[i] = q < n_pieces ? q / per_row : -1;
-      piece[i] = q - (q / per_row) * per_row;
-      dst[i] = (uint32_t)(G_BYTES + (piece[i] >> 2) * BLOCK_BYTES + row[i] * 128);
-    }
-    uint4 code[MAX_P];
-    uint32_t ex[MAX_P];
-    auto request = [&](const Item& m, int kb) {
-#pragma unroll
-      for (int i = 0; i < MAX_P; ++i) {
-        const int64_t r = (int64_t)kb * BK + row[i];
-        const int64_t col = (int64_t)m.kt * p.bn + piece[i] * 16;
-        code[i] = make_uint4(0, 0, 0, 0);
-        ex[i] = 0;
-        if (row[i] >= 0 && r < p.rows && col < p.pitch) {
-          code[i] = *reinterpret_cast<const uint4*>(p.codes + r * p.pitch + col);
-          ex[i] = p.exps[r * (p.pitch / kBlock) + col / kBlock];
-        }
-      }
-    };
-    uint32_t it = 0, chains = 0;
+  } else if (warp < DRAIN0) {
+    // ---------------------------------------------------------------- converters
+    // A piece: 16 codes, two 16-byte chunks of the swizzled tile.  Eight lanes take four pieces of rows r and r ^ 1, whose chunks meet all
+    // banks once; a thread takes every ROWS-th row of its piece's columns.
+    constexpr int LANES = GROUP_WARPS * 32, MAX_PIECES = MAX_BN / CTAS / 16, ROWS = LANES / MAX_PIECES, P = BK / ROWS;
+    const int group = (warp - CONV0) / GROUP_WARPS, t = threadIdx.x - (CONV0 + group * GROUP_WARPS) * 32;
+    const int high = t >> 3, piece = (t & 3) | (high % (MAX_PIECES / 4)) * 4, row = high / (MAX_PIECES / 4) * 2 + ((t >> 2) & 1);
+    const uint32_t dst0 = G_BYTES + (piece >> 2) * BLOCK_BYTES + row * 128 + ((((piece & 3) * 2) ^ (row & 7)) << 4);
+    const bool mine = piece * 16 < own;
+    const int blocks = (int)(p.pitch >> 5);
+    const int64_t code_step = ROWS * p.pitch, code_stage = GROUPS * BK * p.pitch;
+    const int exp_step = ROWS * blocks;
+    const int64_t exp_stage = (int64_t)GROUPS * BK * blocks;
+    uint32_t slot = group, phase = 0;
+    int before = 0;                                  // stages of earlier items, modulo the groups
     bool ok = true;
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    if ((int)blockIdx.x < n_items) {
-      const Item m = item_of(blockIdx.x, p);
-      request(m, m.kb0);
-    }
-    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
+    for (int w = w_first; w < n_items && ok; w += w_step) {
       const Item m = item_of(w, p);
-      for (int kb = m.kb0; kb < m.kb1; ++kb, ++it) {
-        const int s = it % STAGES;
-        if (!mbar_wait_warp(smem_u32(&sh->empty[s]), ((it / STAGES) & 1) ^ 1, abort)) {
+      const int col = m.kt * p.bn + rank * own + piece * 16;
+      const bool there = mine && col < p.pitch;
+      int kb = m.kb0 + (group + GROUPS - before) % GROUPS;
+      before = (before + m.kb1 - m.kb0) % GROUPS;
+      const int64_t r0 = (int64_t)kb * BK + row;
+      const uint8_t* codes = p.codes + r0 * p.pitch + col;
+      const uint8_t* exps = p.exps + r0 * blocks + (col >> 5);
+      for (; kb < m.kb1; kb += GROUPS) {
+        uint4 code[P];
+        uint32_t ex[P];
+        if (there && (kb + 1) * (int64_t)BK <= p.rows) {
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            code[i] = *reinterpret_cast<const uint4*>(codes + i * code_step);
+            ex[i] = exps[i * exp_step];
+          }
+        } else {                                     // the last stage's rows end, or columns past the codes
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const bool live = there && (int64_t)kb * BK + row + i * ROWS < p.rows;
+            code[i] = live ? *reinterpret_cast<const uint4*>(codes + i * code_step) : make_uint4(0, 0, 0, 0);
+            ex[i] = live ? exps[i * exp_step] : 0;
+          }
+        }
+        codes += code_stage;
+        exps += exp_stage;
+        if (!mbar_wait_warp(smem_u32(&sh->empty[slot]), phase ^ 1, abort)) {
           if (lane == 0) give_up(sh, status, 6);
           ok = false;
           break;
         }
+        if (mine) {
+          uint8_t* to = tiles_ptr + slot * STAGE_BYTES + dst0;
+          uint8_t* to2 = tiles_ptr + slot * STAGE_BYTES + (dst0 ^ 16u);
 #pragma unroll
-        for (int i = 0; i < MAX_P; ++i) {
-          if (row[i] >= 0) {
-            const float sc = scale_of(ex[i]);
-            const uint32_t wd[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
-            uint4 o[2];
-            uint32_t* ow = reinterpret_cast<uint32_t*>(o);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float a, b, c, d;
-              decode4<KIND>(wd[j], a, b, c, d);
-              ow[2 * j] = pack2<TG>(a * sc, b * sc);
-              ow[2 * j + 1] = pack2<TG>(c * sc, d * sc);
-            }
-            // the piece's two 16-byte chunks; every other four lanes the second one first, so that eight lanes cover all banks
-            uint8_t* at = tiles_ptr + s * STAGE_BYTES + dst[i];
-            const int c0 = (piece[i] & 3) * 2, flip = (piece[i] >> 2) & 1;
-            *reinterpret_cast<uint4*>(at + (((c0 + flip) ^ (row[i] & 7)) << 4)) = flip ? o[1] : o[0];
-            *reinterpret_cast<uint4*>(at + (((c0 + (flip ^ 1)) ^ (row[i] & 7)) << 4)) = flip ? o[0] : o[1];
+          for (int i = 0; i < P; ++i) {
+            uint32_t o[8];
+            convert16<TG, KIND>(code[i], ex[i], o);
+            *reinterpret_cast<uint4*>(to + i * (ROWS * 128)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(to2 + i * (ROWS * 128)) = make_uint4(o[4], o[5], o[6], o[7]);
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh->full_x[s]));
-        // the next stage's codes
-        if (kb + 1 < m.kb1) {
-          request(m, kb + 1);
-        } else if (w + (int)gridDim.x < n_items) {
-          const Item next = item_of(w + gridDim.x, p);
-          request(next, next.kb0);
+        // one warp's arrival also says that the CTA's part of g has landed
+        if ((warp - CONV0) % GROUP_WARPS == 0 && !mbar_wait_warp(smem_u32(&sh->full_g[slot]), phase, abort)) {
+          if (lane == 0) give_up(sh, status, 7);
+          ok = false;
+          break;
         }
-        const int pos = (kb - m.kb0) % kChain;
-        if (pos == kChain - 1 || kb == m.kb1 - 1) {
-          if (!mbar_wait_warp(smem_u32(&sh->acc_full), chains & 1, abort)) {
-            if (lane == 0) give_up(sh, status, 7);
-            ok = false;
-            break;
-          }
-          ++chains;
-          tc_fence_after();
-          const bool first = kb - m.kb0 < kChain;
-          float* part = p.parts + ((int64_t)m.tile * p.splits + m.split) * (4 * MH * 32) * p.bn;
-          // 32 rows x 32 columns at a time; a lane's row in every column's 128 bytes
-          for (int c = MH == 2 ? 0 : half * 32; c < p.bn; c += MH == 2 ? 32 : 64) {
-            uint32_t r[32];
-            const int h = MH == 2 ? half : 0;
-            tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + h * MAX_BN + c, r);
-            float* out = part + ((int64_t)(h * 4 + quad) * p.bn + c) * 32 + lane;
-            const int cols = min(32, p.bn - c);
-            float old[32];
-            if (!first) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) old[j] = j < cols ? out[j * 32] : 0.f;
-            }
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < cols) out[j * 32] = first ? __uint_as_float(r[j]) : old[j] + __uint_as_float(r[j]);
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sh->acc_empty));
-        }
+        if (lane == 0) arrive_leader(&sh->full_x[slot]);
+        if ((slot += GROUPS) >= STAGES) { slot -= STAGES; phase ^= 1; }
       }
     }
-  } else if (p.bias_parts) {
-    // ---------------------------------------------------------------- column sums of g
-    const int t = threadIdx.x - (2 + CONV_WARPS) * 32;          // 0 .. 127
-    constexpr int CHUNKS = 16 * MH, PHASES = phases_of(MH);
-    const int chunk = t % CHUNKS, phase = t / CHUNKS;           // eight columns, every PHASES-th row; a partial sum each
-    uint32_t it = 0;
+  } else if (warp < SUM0) {
+    // ---------------------------------------------------------------- drain
+    const int quad = warp & 3;                         // TMEM lane quadrant this warp may read
+    uint32_t chains = 0;
     bool ok = true;
-    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
+    for (int w = w_first; w < n_items && ok; w += w_step) {
       const Item m = item_of(w, p);
-      float acc[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-      for (int kb = m.kb0; kb < m.kb1; ++kb, ++it) {
-        const int s = it % STAGES;
-        if (!mbar_wait_warp(smem_u32(&sh->full_g[s]), (it / STAGES) & 1, abort)) {
+      float* part = p.parts + (((int64_t)(m.nt * p.k_tiles + m.kt) * p.splits + m.split) * (4 * CTAS) + rank * 4 + quad) * (p.bn * 32) + lane * 4;
+      for (int kb = m.kb0; kb < m.kb1; kb += kChain, ++chains) {
+        const int buf = chains & 1;
+        if (!mbar_wait_warp(smem_u32(&sh->acc_full[buf]), (chains >> 1) & 1, abort)) {
           if (lane == 0) give_up(sh, status, 8);
           ok = false;
           break;
         }
-        if (m.kt == 0) {
-          const uint8_t* blk = tiles_ptr + s * STAGE_BYTES + (chunk >> 3) * BLOCK_BYTES;
-#pragma unroll 8
-          for (int r = phase; r < BK; r += PHASES) {
-            const uint4 v = *reinterpret_cast<const uint4*>(blk + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
-            float f[8];
-            unpack2<TG>(v.x, f[0], f[1]);
-            unpack2<TG>(v.y, f[2], f[3]);
-            unpack2<TG>(v.z, f[4], f[5]);
-            unpack2<TG>(v.w, f[6], f[7]);
+        tc_fence_after();
+        const bool first = kb == m.kb0;
+        // Four columns of 32 rows are 512 bytes of the workspace.  Later chains are added where they lie: the only additions to an element come
+        // from this thread, in order, so their sum is the same every time, and nothing waits for them (loaded, added and stored the drain took
+        // longer than a chain).
+        for (int c = 0; c < p.bn; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + buf * MAX_BN + c, r);
+          tmem_wait_ld();
+          float* out = part + c * 32;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] += f[j];
+          for (int j = 0; j < 32; j += 4) {
+            if (first) *reinterpret_cast<uint4*>(out + j * 32) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+            else
+              asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(out + j * 32), "f"(__uint_as_float(r[j])),
+                           "f"(__uint_as_float(r[j + 1])), "f"(__uint_as_float(r[j + 2])), "f"(__uint_as_float(r[j + 3]))
+                           : "memory");
           }
         }
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh->empty[s]));
+        if (lane == 0) arrive_leader(&sh->acc_empty[buf]);
+      }
+    }
+  } else if (p.bias_parts) {
+    // ---------------------------------------------------------------- column sums of g
+    constexpr int SG = sum_groups(CTAS), LANES = SUM_WARPS * 32 / SG;          // a group takes every SG-th stage
+    const int t = threadIdx.x - SUM0 * 32, group = t / LANES;
+    const int chunk = t & 15, first = (t % LANES) >> 4;        // eight columns, every (LANES / 16)-th row: a partial sum of its own
+    uint32_t s = 0, phase = 0, turn = 0;
+    bool ok = true;
+    for (int w = w_first; w < n_items && ok; w += w_step) {
+      const Item m = item_of(w, p);
+      float acc[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+      for (int kb = m.kb0; kb < m.kb1; ++kb) {
+        if (turn == group) {
+          if (!mbar_wait_warp(smem_u32(&sh->full_g[s]), phase, abort)) {
+            if (lane == 0) give_up(sh, status, 9);
+            ok = false;
+            break;
+          }
+          if (m.kt == 0) {
+            const uint8_t* blk = tiles_ptr + s * STAGE_BYTES + (chunk >> 3) * BLOCK_BYTES;
+#pragma unroll 8
+            for (int r = first; r < BK; r += LANES / 16) {
+              const uint4 v = *reinterpret_cast<const uint4*>(blk + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+              add_pair<TG>(v.x, acc[0], acc[1]);
+              add_pair<TG>(v.y, acc[2], acc[3]);
+              add_pair<TG>(v.z, acc[4], acc[5]);
+              add_pair<TG>(v.w, acc[6], acc[7]);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh->empty[s]));
+        }
+        if (++turn == SG) turn = 0;
+        if (++s == STAGES) { s = 0; phase ^= 1; }
       }
       if (ok && m.kt == 0) {
-        float4* out = reinterpret_cast<float4*>(p.bias_parts + (((int64_t)m.split * PHASES + phase) * (p.tiles / p.k_tiles) + m.nt) * (128 * MH) + chunk * 8);
+        float4* out = reinterpret_cast<float4*>(p.bias_parts + (((int64_t)m.split * PHASES + (t >> 4)) * p.n_tiles + m.nt) * (128 * CTAS) + rank * 128 + chunk * 8);
         out[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
         out[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
       }
@@ -327,59 +427,71 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
   pdl_trigger();
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();          // nothing is signalled to, or read from, a CTA that has left
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+    PAIR ? tmem_dealloc_pair(tmem_base, TMEM_COLS) : tmem_dealloc(tmem_base, TMEM_COLS);
   }
 }
 
-// Adds the partial tiles in the order of their rows: a block takes 32 x 32 of the weight (or, past those, 256 of the bias).
+// Adds the partial tiles in the order of their rows: a block takes 32 x 32 of the weight (or, past those, 32 of the bias).
 struct AddArgs {
   const float* parts;
   const float* bias_parts;
   float* gw;
   float* gb;
   int64_t ldw;
-  int n, k, bn, k_tiles, tiles, splits, mh;
+  int n, k, bn, n_tiles, k_tiles, splits, ctas;
   int64_t patches;
 };
 __global__ void __launch_bounds__(256) wgrad8_add_kernel(AddArgs p) {
   pdl_begin();
-  if (blockIdx.x >= p.patches) {
-    const int c = (int)(blockIdx.x - p.patches) * 256 + threadIdx.x, width = p.tiles / p.k_tiles * 128 * p.mh;
+  __shared__ float patch[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x >= p.patches) {             // 32 columns of g: a warp takes every eighth partial sum, then the warps' sums in order
+    const int c = (int)(blockIdx.x - p.patches) * 32 + lane, width = p.n_tiles * 128 * p.ctas;
+    float sum = 0.f;
     if (c < p.n) {
-      float sum = 0.f;
 #pragma unroll 8
-      for (int s = 0; s < p.splits * phases_of(p.mh); ++s) sum += p.bias_parts[(int64_t)s * width + c];
+      for (int s = warp; s < p.splits * PHASES; s += 8) sum += p.bias_parts[(int64_t)s * width + c];
+    }
+    patch[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && c < p.n) {
+#pragma unroll
+      for (int w = 1; w < 8; ++w) sum += patch[w][lane];
       p.gb[c] = sum;
     }
     return;
   }
-  __shared__ float patch[32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int chunks = (p.bn + 31) / 32, blocks = 4 * p.mh;
+  const int chunks = p.bn / 32, blocks = 4 * p.ctas;
   int64_t i = blockIdx.x;
   const int chunk = (int)(i % chunks);
   i /= chunks;
   const int blk = (int)(i % blocks), tile = (int)(i / blocks);
   const int64_t slot = (int64_t)blocks * p.bn * 32;
-  const float* from = p.parts + (int64_t)tile * p.splits * slot + ((int64_t)blk * p.bn + chunk * 32) * 32 + lane;
-  const int cols = min(32, p.bn - chunk * 32);
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < p.splits; ++s)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (warp + 8 * j < cols) sum[j] += from[s * slot + (warp + 8 * j) * 32];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) patch[warp + 8 * j][lane] = sum[j];
+  // thread: row `lane` of four columns (bn is a multiple of 32)
+  const float4* from = reinterpret_cast<const float4*>(p.parts + (int64_t)tile * p.splits * slot + ((int64_t)blk * p.bn + chunk * 32) * 32 + warp * 128) + lane;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int s = 0; s < p.splits; ++s) {
+    const float4 v = from[s * (slot / 4)];
+    sum.x += v.x;
+    sum.y += v.y;
+    sum.z += v.z;
+    sum.w += v.w;
+  }
+  patch[warp * 4][lane] = sum.x;
+  patch[warp * 4 + 1][lane] = sum.y;
+  patch[warp * 4 + 2][lane] = sum.z;
+  patch[warp * 4 + 3][lane] = sum.w;
   __syncthreads();
   const int nt = tile / p.k_tiles, kt = tile % p.k_tiles;
   const int col = kt * p.bn + chunk * 32 + lane;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int row = nt * 128 * p.mh + blk * 32 + warp + 8 * j;
-    if (row < p.n && col < p.k && lane < cols) p.gw[(int64_t)row * p.ldw + col] = patch[lane][warp + 8 * j];
+    const int row = nt * 128 * p.ctas + blk * 32 + warp + 8 * j;
+    if (row < p.n && col < p.k) p.gw[(int64_t)row * p.ldw + col] = patch[lane][warp + 8 * j];
   }
 }
 
@@ -393,7 +505,7 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* __restr
 
 // How a call is cut up
 struct Plan {
-  int mh, bn, k_tiles, tiles, splits, k_blocks;
+  int ctas, bn, n_tiles, k_tiles, splits, k_blocks;
   bool copy;
   int64_t copy_bytes, parts_bytes, bias_bytes;
 };
@@ -403,36 +515,37 @@ Plan plan_of(int64_t rows, int n, int k, bool copy) {
   best.copy = copy;
   const int sms = sm_count();
   double cost = 1e30;
-  for (int mh = 1; mh <= 2; ++mh)
+  for (int ctas = 1; ctas <= 2; ++ctas)
     for (int most = 64; most <= MAX_BN; most *= 2) {
-      const int k_tiles = (k + most - 1) / most, bn = (int)round_up((k + k_tiles - 1) / k_tiles, 16);
-      const int64_t tiles = (int64_t)((n + 128 * mh - 1) / (128 * mh)) * k_tiles;
+      const int k_tiles = (k + most - 1) / most, bn = (int)round_up((k + k_tiles - 1) / k_tiles, 32 * ctas);
+      const int n_tiles = (n + 128 * ctas - 1) / (128 * ctas), units = sms / ctas;
+      const int64_t tiles = (int64_t)n_tiles * k_tiles;
       if (tiles > 1 << 20) continue;
-      // cycles of a stage: conversions, MMAs with their operand reads; of a drain; of the partial tiles' way to memory and back, all SMs
-      const double stage = fmax(2.2 * bn, fmax(4.0 * mh * 0.65 * bn, 140.0)), drain = 1500 + 24.0 * mh * bn;
+      // cycles of a stage and of a drain that nothing hides (an item's last); bytes of partial tiles, all SMs
+      const double stage = fmax(ctas == 2 ? 3.1 * bn : 4.0 * bn, 400.0), drain = 2000 + 12.0 * bn;
       // pieces of the rows: as fill one or more waves of SMs, or stages of some length each
       for (int i = 0; i < 10; ++i) {
-        int64_t splits = i < 4 ? (i + 1) * (int64_t)sms / tiles : best.k_blocks >> (i - 4);
+        int64_t splits = i < 4 ? (i + 1) * (int64_t)units / tiles : best.k_blocks >> (i - 4);
         splits = splits < 1 ? 1 : splits > best.k_blocks ? best.k_blocks : splits;
         if (splits > 2 * sms) continue;
-        const double waves = (double)((tiles * splits + sms - 1) / sms), per = (double)((best.k_blocks + splits - 1) / splits);
-        const double c = waves * (per * stage + drain * ceil(per / kChain)) + (double)tiles * splits * 128 * mh * bn * 4 / 5000.0;
+        const double waves = (double)((tiles * splits + units - 1) / units), per = (double)((best.k_blocks + splits - 1) / splits);
+        const double c = waves * per * stage + drain + (double)tiles * splits * 128 * ctas * bn * 4 / 5000.0;
         if (c < cost) {
           cost = c;
-          best.mh = mh; best.bn = bn; best.k_tiles = k_tiles; best.tiles = (int)tiles; best.splits = (int)splits;
+          best.ctas = ctas; best.bn = bn; best.n_tiles = n_tiles; best.k_tiles = k_tiles; best.splits = (int)splits;
         }
       }
     }
   best.copy_bytes = copy ? round_up(rows * round_up(n, 8) * 2, 256) : 0;
-  best.parts_bytes = round_up((int64_t)best.tiles * best.splits * 128 * best.mh * best.bn * 4, 256);
-  best.bias_bytes = round_up((int64_t)best.splits * phases_of(best.mh) * (best.tiles / best.k_tiles) * 128 * best.mh * 4, 256);
+  best.parts_bytes = round_up((int64_t)best.n_tiles * best.k_tiles * best.splits * 128 * best.ctas * best.bn * 4, 256);
+  best.bias_bytes = round_up((int64_t)best.splits * PHASES * best.n_tiles * 128 * best.ctas * 4, 256);
   return best;
 }
 
 template <typename TG, int KIND>
 void launch(const Plan& pl, const CUtensorMap& tm, const Args& p, int* status, cudaStream_t stream) {
-  const int items = p.tiles * p.splits, grid = items < sm_count() ? items : sm_count();
-  if (pl.mh == 2) launch_kernel(wgrad8_kernel<TG, KIND, 2>, grid, THREADS, smem_bytes(2), stream, tm, p, status);
+  const int items = p.n_tiles * p.k_tiles * p.splits, units = sm_count() / pl.ctas, grid = (items < units ? items : units) * pl.ctas;
+  if (pl.ctas == 2) launch_kernel<2>(wgrad8_kernel<TG, KIND, 2>, grid, THREADS, smem_bytes(2), stream, tm, p, status);
   else launch_kernel(wgrad8_kernel<TG, KIND, 1>, grid, THREADS, smem_bytes(1), stream, tm, p, status);
 }
 bool needs_copy(const void* g, int64_t ldg) { return !aligned16(g) || ldg % 8 != 0; }
@@ -464,7 +577,7 @@ int wgrad8(const void* g, int g_dtype, int64_t ldg, const uint8_t* codes, const 
   float* bias_parts = gb ? reinterpret_cast<float*>(ws + pl.copy_bytes + pl.parts_bytes) : nullptr;
   CUtensorMap tm;
   if (!make_tmap_f16(&tm, g, rows, n, ldg, BK)) return BSRL_ERR_CUDA;
-  const Args p{codes, exps, rows, pitch_of(k), n, pl.bn, pl.k_tiles, pl.tiles, pl.splits, pl.k_blocks, parts, bias_parts};
+  const Args p{codes, exps, rows, pitch_of(k), pl.bn, pl.n_tiles, pl.k_tiles, pl.splits, pl.k_blocks, parts, bias_parts};
   static DeviceOnce once;
   const int rc = once.run("wgrad8_kernel set-up", [] {
     cudaError_t e = cudaSuccess;
@@ -480,11 +593,11 @@ int wgrad8(const void* g, int g_dtype, int64_t ldg, const uint8_t* codes, const 
   if (g_dtype == BSRL_F16) kind == kInt8 ? launch<__half, kInt8>(pl, tm, p, status, stream) : launch<__half, kE4m3>(pl, tm, p, status, stream);
   else kind == kInt8 ? launch<__nv_bfloat16, kInt8>(pl, tm, p, status, stream) : launch<__nv_bfloat16, kE4m3>(pl, tm, p, status, stream);
   BSRL_LAUNCH_OK("wgrad8_kernel");
-  AddArgs a{parts, bias_parts, gw, gb, ldw, n, k, pl.bn, pl.k_tiles, pl.tiles, pl.splits, pl.mh, 0};
-  a.patches = (int64_t)pl.tiles * 4 * pl.mh * ((pl.bn + 31) / 32);
+  AddArgs a{parts, bias_parts, gw, gb, ldw, n, k, pl.bn, pl.n_tiles, pl.k_tiles, pl.splits, pl.ctas, 0};
+  a.patches = (int64_t)pl.n_tiles * pl.k_tiles * 4 * pl.ctas * (pl.bn / 32);
   PdlScope overlap;
   pdl_enable();
-  launch_kernel(wgrad8_add_kernel, (unsigned)(a.patches + (gb ? (n + 255) / 256 : 0)), 256, 0, stream, a);
+  launch_kernel(wgrad8_add_kernel, (unsigned)(a.patches + (gb ? (n + 31) / 32 : 0)), 256, 0, stream, a);
   BSRL_LAUNCH_OK("wgrad8_add_kernel");
   return BSRL_OK;
 }
