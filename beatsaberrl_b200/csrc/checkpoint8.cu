@@ -29,7 +29,7 @@ int check_rows(const char* what, const void* p, int dtype, int64_t ld, int64_t r
 int check_kept(const char* what, const uint8_t* codes, const uint8_t* exps, int kind, int64_t rows) {
   if (kind != BSRL_INT8 && kind != BSRL_E4M3) return refuse(BSRL_ERR_UNSUPPORTED, what, "the kind must be BSRL_INT8 or BSRL_E4M3");
   if (rows > 0 && (!codes || !exps)) return refuse(BSRL_ERR_NULL, what, "NULL codes or exps");
-  if (!aligned16(codes)) return refuse(BSRL_ERR_ALIGN, what, "codes must be 16-byte aligned");
+  if (!aligned16(codes) || !aligned_to(exps, 4)) return refuse(BSRL_ERR_ALIGN, what, "codes must be 16-byte, exps 4-byte aligned");
   return BSRL_OK;
 }
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
@@ -91,7 +91,7 @@ int bsrl_layernorm8(const void* x, const void* residual, int32_t dtype, int64_t 
     CHECK(check_rows(me, z, dtype, ldz, rows, d));
   }
   CHECK(check_kept(me, codes, exps, kind, rows));
-  if (d > norm8_max_width()) return refuse(BSRL_ERR_SHAPE, me, "rows are at most 16,384 wide");
+  if (d > norm8_max_width()) return refuse(BSRL_ERR_SHAPE, me, "rows are at most 8,192 wide");
   if (!norm8_types_ok(dtype, y_dtype)) return refuse(BSRL_ERR_UNSUPPORTED, me, "16-bit rows give results of their own type");
   if (!gamma || (rows > 0 && (!mean || !rstd))) return refuse(BSRL_ERR_NULL, me, "NULL gamma, mean or rstd");
   if (!aligned_to(gamma, 4) || !aligned_to(beta, 4) || !aligned_to(mean, 4) || !aligned_to(rstd, 4))
@@ -103,7 +103,7 @@ int bsrl_layernorm8(const void* x, const void* residual, int32_t dtype, int64_t 
 
 int64_t bsrl_layernorm8_bwd_workspace_bytes(int64_t rows, int32_t d) {
   if (rows < 0 || d < 1 || d > norm8_max_width()) {
-    set_error("layernorm8_bwd: rows must not be negative, the width 1 .. 16,384");
+    set_error("layernorm8_bwd: rows must not be negative, the width 1 .. 8,192");
     return -1;
   }
   return norm8_bwd_workspace(rows, d);
@@ -118,7 +118,7 @@ int bsrl_layernorm8_bwd(const void* gy, int32_t gy_dtype, int64_t ldgy, const vo
   CHECK(check_rows(me, gx, dtype, ldgx, rows, d));
   if (g_residual) CHECK(check_rows(me, g_residual, dtype, ldgr, rows, d));
   CHECK(check_kept(me, codes, exps, kind, rows));
-  if (d > norm8_max_width()) return refuse(BSRL_ERR_SHAPE, me, "rows are at most 16,384 wide");
+  if (d > norm8_max_width()) return refuse(BSRL_ERR_SHAPE, me, "rows are at most 8,192 wide");
   if (!norm8_types_ok(dtype, gy_dtype)) return refuse(BSRL_ERR_UNSUPPORTED, me, "16-bit rows take gradients of their own type");
   if (!gamma || (rows > 0 && (!mean || !rstd))) return refuse(BSRL_ERR_NULL, me, "NULL gamma, mean or rstd");
   if (!aligned_to(gamma, 4) || !aligned_to(g_gamma, 4) || !aligned_to(g_beta, 4) || !aligned_to(mean, 4) || !aligned_to(rstd, 4))

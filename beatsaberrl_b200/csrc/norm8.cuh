@@ -6,8 +6,12 @@
 //   g_gamma = sum over rows of gy h,  g_beta = sum over rows of gy
 //
 // Streams: per element of fp32 rows with fp16 outputs 7 1/32 bytes forward and 7 1/32 backward.  A row belongs to a team of lanes -- 4, 8, 16 or 32
-// of a warp up to 1024 columns, a whole block above -- which holds it in registers between its one read and its one write, eight
-// neighbouring elements per lane and step (16-byte accesses).  Rows that 16 bytes do not divide go one element per lane.
+// of a warp up to 512 columns, a whole block above -- which holds it in registers between its one read and its one write, eight
+// neighbouring elements per lane and step.  Rows that 16 bytes do not divide are read by the aligned 16 bytes around a lane's piece and shifted
+// into place, and written the same way with the end of the neighbouring lane's piece.
+// 475,136 fp32 rows of 256 with fp16 results: 140 us forward (94 % of the copy rate), 163 backward (81 %).  What bounds the backward is the
+// instructions (220 per row and warp) and the 16 warps that its registers leave.  With twice the instructions (arithmetic one element at a
+// time, IEEE divisions) both took over 200 us whatever was requested ahead, in registers or through a ring in shared memory.
 //
 // The parameter gradients are summed in one order: every lane adds the rows it meets into registers, a block's teams add up through
 // shared memory one after the other, blocks write partial rows and a second kernel adds those in order.  No atomics, so a call gives the same
@@ -50,158 +54,224 @@ struct BwdArgs {
   int d, kind;
 };
 
-// Sums over a team's lanes.  TPR > 0: TPR lanes of a warp.  TPR = 0 (-1): a block of up to 512 (1024) threads; `turn` alternates between two sets of shared slots, so
-// that one barrier per sum is enough.
-template <int TPR>
-__device__ __forceinline__ void team_sum(float& a, float& b, float2 (*slots)[32], int& turn) {
+// Sums of N numbers over a team's lanes.  TPR > 0: TPR lanes of a warp.  TPR = 0: the block; `turn` alternates between two sets of shared
+// slots, so that one barrier per sum is enough.
+template <int TPR, int N>
+__device__ __forceinline__ void team_sum(float (&a)[N], float (*slots)[32][4], int& turn) {
   constexpr int W = TPR > 0 ? TPR : 32;
 #pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
-  if constexpr (TPR <= 0) {
-    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) slots[turn][threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    const float2 s = lane < warps ? slots[turn][lane] : make_float2(0.f, 0.f);
-    a = s.x;
-    b = s.y;
+  for (int o = W / 2; o > 0; o >>= 1)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
+    for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], o);
+  if constexpr (TPR == 0) {
+    static_assert(N <= 4, "");
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) slots[turn][threadIdx.x >> 5][i] = a[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = lane < warps ? slots[turn][lane][i] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], o);
     turn ^= 1;
   }
 }
 
-template <int V>
-__device__ __forceinline__ void load_f32(const float* p, float (&v)[V]) {
-  Raw<float, V> r;
-  r.load(p);
-  r.get(v);
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+template <bool ALIGNED, typename T>
+__device__ __forceinline__ void load_piece(Raw8<T>& r, const T* p, int n, const Span& s) {
+  if (ALIGNED) r.load(p);
+  else load_any(r, p, n, s);
+}
+// eight of a parameter's d values
+template <bool ALIGNED>
+__device__ __forceinline__ Eight load_param(const float* p, int col, int d) {
+  Raw8<float> r;
+  load_piece<ALIGNED>(r, p + col, d - col, ALIGNED ? Span{} : span_of(p, 1, d, d));
+  return Eight::of(r);
+}
+// Writes step i of a row.  `last`: the words of the step ahead, whose last lane's end lane 0 needs (a team of a warp's lanes; a block's warps
+// write their edges element by element).  All lanes call it.
+template <bool ALIGNED, int TPR, typename T>
+__device__ __forceinline__ void store_piece(const Raw8<T>& r, T* row, int piece, int d, bool live, uint32_t (&last)[4]) {
+  const int col = piece * 8;
+  if (ALIGNED) {
+    if (live && col < d) r.store(row + col);
+    return;
+  }
+  constexpr int W = Raw8<T>::kWords, TEAM = TPR > 0 ? TPR : 32;
+  const int lane = threadIdx.x & 31, in_team = lane % TEAM;
+  uint32_t prev[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t mine = r.w[W - 4 + j];
+    prev[j] = __shfl_sync(0xffffffffu, TPR > 0 && in_team == TEAM - 1 ? last[j] : mine, (lane - in_team) + (in_team + TEAM - 1) % TEAM);
+    last[j] = mine;
+  }
+  const bool ahead = TPR > 0 ? piece > 0 : in_team > 0, behind = (TPR > 0 || in_team < TEAM - 1) && col + 16 <= d;
+  if (live && col < d) store_any(r, row + col, d - col, prev, ahead, behind);
 }
 
-constexpr int kThreads = 256;
-constexpr int block_threads(int tpr) { return tpr > 0 ? kThreads : tpr == 0 ? 512 : 1024; }
-// blocks of kThreads per SM that the kernels are built for, by what a lane holds
-constexpr int fwd_resident(int held) { return held <= 8 ? 5 : held <= 16 ? 3 : 2; }
-constexpr int bwd_resident(int held) { return held <= 8 ? 4 : held <= 16 ? 2 : 1; }
+constexpr int kThreads = 256;                      // of blocks whose warps hold teams
+constexpr int block_threads(int tpr) { return tpr > 0 ? kThreads : 512; }
+// blocks of kThreads per SM: 128 registers each.  Three forward (80 registers, spills) 213 us where two are 176, of 475,136 rows of 256
+constexpr int kResident = 2;
 
-// R: rows a team has in flight.  NV: steps of V elements that a lane takes of a row.
-template <typename T, typename TY, int V, int TPR, int NV, int R>
-__global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? fwd_resident(NV * V * R) : 1) norm8_fwd_kernel(FwdArgs<T, TY> p) {
-  __shared__ float2 slots[2][32];
-  int turn = 0;
-  constexpr int W = TPR > 0 ? TPR : 32;
-  const int lane = threadIdx.x & 31;
-  const int at = TPR > 0 ? lane % W : threadIdx.x, stride = TPR > 0 ? W : blockDim.x;       // this lane's pieces of a row: at + i stride
-  constexpr int TEAMS = TPR > 0 ? 32 / W : 1;
-  const int team = TPR > 0 ? lane / W : 0;
-  const int d = p.d, pitch = (int)pitch_of(d);
-  const int64_t first = TPR > 0 ? ((int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * (TEAMS * R) : blockIdx.x;
-  const int64_t step = TPR > 0 ? (int64_t)gridDim.x * (blockDim.x >> 5) * (TEAMS * R) : gridDim.x;
-  pdl_begin();
-  float g1[V], b1[V];
-  if (NV == 1) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) g1[j] = b1[j] = 0.f;
-    if (at * V < d) {
-      load_f32<V>(p.gamma + at * V, g1);
-      if (p.beta) load_f32<V>(p.beta + at * V, b1);
-    }
+// This thread's part of the rows.  TPR > 0: TPR lanes of a warp hold a row; TPR = 0: the block does.  A warp or block takes ROWS rows at a time.
+template <int TPR, int R>
+struct Place {
+  static constexpr int TEAM = TPR > 0 ? TPR : 32, TEAMS = TPR > 0 ? 32 / TEAM : 1, ROWS = TEAMS * R;
+  int at, stride, team;          // the lane's pieces of a row: at + i stride
+  int64_t first, step;
+  __device__ __forceinline__ Place() {
+    const int lane = threadIdx.x & 31;
+    at = TPR > 0 ? lane % TEAM : threadIdx.x;
+    stride = TPR > 0 ? TEAM : blockDim.x;
+    team = TPR > 0 ? lane / TEAM : 0;
+    first = TPR > 0 ? ((int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * ROWS : (int64_t)blockIdx.x * ROWS;
+    step = TPR > 0 ? (int64_t)gridDim.x * (blockDim.x >> 5) * ROWS : (int64_t)gridDim.x * ROWS;
   }
-  for (int64_t base = first; base < p.rows; base += step) {
-    Raw<T, V> raw[R][NV], rres[R][NV];
+};
+
+// R: rows a team works on together.  NV: steps of eight elements that a lane takes of a row.  RES: there is a residual.
+template <typename T, typename TY, bool ALIGNED, bool RES, int TPR, int NV, int R>
+__global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? kResident : 1) norm8_fwd_kernel(FwdArgs<T, TY> p) {
+  __shared__ float slots[2][32][4];
+  int turn = 0;
+  const Place<TPR, R> pl;
+  const int at = pl.at, stride = pl.stride, d = p.d, pitch = (int)pitch_of(d);
+  const bool res = RES && (ALIGNED || p.res);      // the kernels of unaligned rows have one form
+  const Span span_x = ALIGNED ? Span{} : span_of(p.x, p.rows, d, p.ldx), span_r = ALIGNED || !res ? Span{} : span_of(p.res, p.rows, d, p.ldr);
+  const float inv_d = 1.f / d;
+  pdl_begin();
+  Eight g1 = Eight::all(0.f), b1 = g1;
+  if (NV == 1 && at * 8 < d) {
+    g1 = load_param<ALIGNED>(p.gamma, at * 8, d);
+    if (p.beta) b1 = load_param<ALIGNED>(p.beta, at * 8, d);
+  }
+  for (int64_t base = pl.first; base < p.rows; base += pl.step) {
+    Raw8<T> x[R][NV], r2[R][NV];
+    bool live[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * TEAMS + team;
+      const int64_t row = base + r * pl.TEAMS + pl.team;
+      live[r] = row < p.rows;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int col = (at + i * stride) * V;
-        if (row < p.rows && col < d) {
-          raw[r][i].load(p.x + row * p.ldx + col);
-          if (p.res) rres[r][i].load(p.res + row * p.ldr + col);
-        } else {
-          raw[r][i].zero();
-          rres[r][i].zero();
+        const int col = (at + i * stride) * 8;
+        x[r][i].zero();
+        if (RES) r2[r][i].zero();
+        if (live[r] && col < d) {
+          load_piece<ALIGNED>(x[r][i], p.x + row * p.ldx + col, d - col, span_x);
+          if (res) load_piece<ALIGNED>(r2[r][i], p.res + row * p.ldr + col, d - col, span_r);
         }
       }
     }
+    // the next rows, into L2: no registers, and half of the latency (176 -> 141 us, backward 218 -> 167 of 475,136 rows of 256)
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * TEAMS + team;
-      const bool live = row < p.rows;
-      float v[NV][V];
-      float s = 0.f, q = 0.f;
+      const int64_t row = base + pl.step + r * pl.TEAMS + pl.team;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int col = (at + i * stride) * V;
-        raw[r][i].get(v[i]);
-        if (p.res) {
-          float w[V];
-          rres[r][i].get(w);
-#pragma unroll
-          for (int j = 0; j < V; ++j) v[i][j] += w[j];
-          raw[r][i].set(v[i]);
-          raw[r][i].get(v[i]);                     // as the stream has it: rounded to its type
-          if (live && col < d && p.z) raw[r][i].store(p.z + row * p.ldz + col);
+        const int col = (at + i * stride) * 8;
+        if (row < p.rows && col < d) {
+          prefetch_l2(p.x + row * p.ldx + col);
+          if (res) prefetch_l2(p.res + row * p.ldr + col);
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) s += v[i][j];
       }
-      float none = 0.f;
-      team_sum<TPR>(s, none, slots, turn);
-      const float mean = s / d;
+    }
+    float sum[R], var[R];
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if ((at + i * stride) * V < d) {
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + r * pl.TEAMS + pl.team;
+      sum[r] = var[r] = 0.f;
+      uint32_t last[4] = {};
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float c = v[i][j] - mean;
-            q = fmaf(c, c, q);
-          }
+      for (int i = 0; i < NV; ++i) {
+        Eight v = Eight::of(x[r][i]);
+        if (RES) {
+          const Eight w = Eight::of(r2[r][i]);
+          float f[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v.p[j] = f2_add(v.p[j], w.p[j]);
+          v.split(f);
+          x[r][i].set(f);
+          v = Eight::of(x[r][i]);                  // as the stream has it: rounded to its type
+          if (res) store_piece<ALIGNED, TPR>(x[r][i], p.z + row * p.ldz, at + i * stride, d, live[r], last);
         }
-      team_sum<TPR>(q, none, slots, turn);
-      const float rstd = 1.f / sqrtf(q / d + p.eps);
-      if (at == 0 && live) {
-        p.mean[row] = mean;
+        sum[r] += v.sum();
+      }
+    }
+    team_sum<TPR>(sum, slots, turn);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      sum[r] *= inv_d;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (at + i * stride) * 8;
+        Eight v = Eight::of(x[r][i]), q = Eight::all(0.f);
+        const Eight m = Eight::all(-sum[r]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v.p[j] = f2_add(v.p[j], m.p[j]);
+        if (!ALIGNED && col + 8 > d) {             // elements that the row does not have
+          float f[8];
+          v.split(f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = col + j < d ? f[j] : 0.f;
+          v = Eight::of(f);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q.p[j] = f2_mul(v.p[j], v.p[j]);
+        if (col < d) var[r] += q.sum();
+      }
+    }
+    team_sum<TPR>(var, slots, turn);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + r * pl.TEAMS + pl.team;
+      const float rstd = rsqrtf(fmaf(var[r], inv_d, p.eps));
+      if (at == 0 && live[r]) {
+        p.mean[row] = sum[r];
         p.rstd[row] = rstd;
       }
+      uint32_t last[4] = {};
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int col = (at + i * stride) * V;
-        if (live && col < d) {
-          float g[V], b[V], o[V];
-          if (NV == 1) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) g[j] = g1[j], b[j] = b1[j];
-          } else {
-            load_f32<V>(p.gamma + col, g);
-            if (p.beta) load_f32<V>(p.beta + col, b);
-            else
-#pragma unroll
-              for (int j = 0; j < V; ++j) b[j] = 0.f;
+        const int col = (at + i * stride) * 8;
+        Eight v = Eight::of(x[r][i]);
+        Raw8<TY> out;
+        out.zero();
+        if (live[r] && col < d) {
+          Eight g = g1, b = b1;
+          if (NV > 1) {
+            g = load_param<ALIGNED>(p.gamma, col, d);
+            if (p.beta) b = load_param<ALIGNED>(p.beta, col, d);
           }
+          const Eight m = Eight::all(-sum[r]), s = Eight::all(rstd);
+          Eight o;
 #pragma unroll
-          for (int j = 0; j < V; ++j) o[j] = fmaf((v[i][j] - mean) * rstd, g[j], b[j]);
-          Raw<TY, V> out;
-          out.set(o);
-          out.store(p.y + row * p.ldy + col);
+          for (int j = 0; j < 4; ++j) o.p[j] = f2_fma(f2_mul(f2_add(v.p[j], m.p[j]), s.p[j]), g.p[j], b.p[j]);
+          float f[8];
+          o.split(f);
+          out.set(f);
         }
-        float inv;
-        const uint32_t bits = block_max_bits<V>(v[i]);
-        Codes<V> c;
+        store_piece<ALIGNED, TPR>(out, p.y + row * p.ldy, at + i * stride, d, live[r], last);
+        float f[8], inv;
+        v.split(f);
+        const uint32_t bits = block_max_bits(f);
+        Codes c;
         uint32_t e;
         if (p.kind == kInt8) {
-          e = block_exp<T, kInt8, V>(bits, v[i], inv);
-          encode<kInt8>(v[i], inv, c);
+          e = block_exp<T, kInt8>(bits, f, inv);
+          encode<kInt8>(f, inv, c);
         } else {
-          e = block_exp<T, kE4m3, V>(bits, v[i], inv);
-          encode<kE4m3>(v[i], inv, c);
+          e = block_exp<T, kE4m3>(bits, f, inv);
+          encode<kE4m3>(f, inv, c);
         }
-        if (live && col < pitch) {
+        if (live[r] && col < pitch) {
           c.store(p.codes + row * pitch + col);
           if (col % kBlock == 0) p.exps[row * (pitch / kBlock) + col / kBlock] = (uint8_t)e;
         }
@@ -210,162 +280,177 @@ __global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? fwd_resident(NV 
   }
 }
 
-template <typename T, typename TY, int V, int TPR, int NV, int R>
-__global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? bwd_resident(NV * V * R) : 1) norm8_bwd_kernel(BwdArgs<T, TY> p) {
-  __shared__ float2 slots[2][32];
+template <typename T, typename TY, bool ALIGNED, bool RES, int TPR, int NV, int R>
+__global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? kResident : 1) norm8_bwd_kernel(BwdArgs<T, TY> p) {
+  __shared__ float slots[2][32][4];
   extern __shared__ float s_sums[];                  // [2][d], teams of lanes only
   int turn = 0;
-  constexpr int W = TPR > 0 ? TPR : 32;
-  const int lane = threadIdx.x & 31;
-  const int at = TPR > 0 ? lane % W : threadIdx.x, stride = TPR > 0 ? W : blockDim.x;
-  constexpr int TEAMS = TPR > 0 ? 32 / W : 1;
-  const int team = TPR > 0 ? lane / W : 0;
-  const int d = p.d, pitch = (int)pitch_of(d), blocks = pitch / kBlock;
-  const int64_t first = TPR > 0 ? ((int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * (TEAMS * R) : blockIdx.x;
-  const int64_t step = TPR > 0 ? (int64_t)gridDim.x * (blockDim.x >> 5) * (TEAMS * R) : gridDim.x;
+  const Place<TPR, R> pl;
+  const int at = pl.at, stride = pl.stride, d = p.d, pitch = (int)pitch_of(d), blocks = pitch / kBlock;
+  const bool res = RES && (ALIGNED || p.gres);
+  const Span span_g = ALIGNED ? Span{} : span_of(p.gy, p.rows, d, p.ldgy), span_r = ALIGNED || !res ? Span{} : span_of(p.gres, p.rows, d, p.ldgr);
   const float inv_d = 1.f / d;
   pdl_begin();
-  float g1[V];
-  if (NV == 1) {
+  Eight g1 = Eight::all(0.f);
+  if (NV == 1 && at * 8 < d) g1 = load_param<ALIGNED>(p.gamma, at * 8, d);
+  Eight acc_g[NV], acc_b[NV];
 #pragma unroll
-    for (int j = 0; j < V; ++j) g1[j] = 0.f;
-    if (at * V < d) load_f32<V>(p.gamma + at * V, g1);
-  }
-  float acc_g[NV][V], acc_b[NV][V];
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc_g[i][j] = acc_b[i][j] = 0.f;
-  for (int64_t base = first; base < p.rows; base += step) {
-    Raw<TY, V> rgy[R][NV];
-    Raw<T, V> rres[R][NV];
-    Codes<V> codes[R][NV];
+  for (int i = 0; i < NV; ++i) acc_g[i] = acc_b[i] = Eight::all(0.f);
+  for (int64_t base = pl.first; base < p.rows; base += pl.step) {
+    Raw8<TY> gy[R][NV];
+    Raw8<T> r2[R][NV];
+    Codes codes[R][NV];
     uint32_t exps[R][NV];
     float mean[R], rstd[R];
+    bool live[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * TEAMS + team;
-      const bool live = row < p.rows;
-      mean[r] = live ? p.mean[row] : 0.f;
-      rstd[r] = live ? p.rstd[row] : 0.f;
+      const int64_t row = base + r * pl.TEAMS + pl.team;
+      live[r] = row < p.rows;
+      mean[r] = rstd[r] = 0.f;
+      if (live[r]) {
+        mean[r] = p.mean[row];
+        rstd[r] = p.rstd[row];
+      }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int col = (at + i * stride) * V;
-        if (live && col < d) {
-          rgy[r][i].load(p.gy + row * p.ldgy + col);
+        const int col = (at + i * stride) * 8;
+        gy[r][i].zero();
+        codes[r][i].zero();
+        exps[r][i] = 0;
+        if (RES) r2[r][i].zero();
+        if (live[r] && col < d) {
+          load_piece<ALIGNED>(gy[r][i], p.gy + row * p.ldgy + col, d - col, span_g);
           codes[r][i].load(p.codes + row * pitch + col);
           exps[r][i] = p.exps[row * blocks + col / kBlock];
-          if (p.gres) rres[r][i].load(p.gres + row * p.ldgr + col);
-        } else {
-          rgy[r][i].zero();
-          codes[r][i].zero();
-          exps[r][i] = 0;
+          if (res) load_piece<ALIGNED>(r2[r][i], p.gres + row * p.ldgr + col, d - col, span_r);
         }
       }
     }
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * TEAMS + team;
-      const bool live = row < p.rows;
-      // h of one step: the codes' scale and the row's rstd in one factor
-      const float shift = -mean[r] * rstd[r];
-      auto hidden = [&](int i, float (&h)[V]) {
-        if (p.kind == kInt8) decode<kInt8>(codes[r][i], h);
-        else decode<kE4m3>(codes[r][i], h);
-        const float s = scale_of(exps[r][i]);
-#pragma unroll
-        for (int j = 0; j < V; ++j) h[j] = fmaf(h[j] * s, rstd[r], shift);
-      };
-      float s1 = 0.f, s2 = 0.f;
+    for (int r = 0; r < R; ++r) {                      // the next rows, into L2
+      const int64_t row = base + pl.step + r * pl.TEAMS + pl.team;
+      if (at == 0 && row < p.rows) {
+        prefetch_l2(p.mean + row);
+        prefetch_l2(p.rstd + row);
+        prefetch_l2(p.exps + row * blocks);
+      }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int col = (at + i * stride) * V;
-        if (live && col < d) {
-          float h[V], g[V], gm[V];
-          hidden(i, h);
-          rgy[r][i].get(g);
-          if (NV == 1) {
+        const int col = (at + i * stride) * 8;
+        if (row < p.rows && col < d) {
+          prefetch_l2(p.gy + row * p.ldgy + col);
+          prefetch_l2(p.codes + row * pitch + col);
+          if (res) prefetch_l2(p.gres + row * p.ldgr + col);
+        }
+      }
+    }
+    // rows one after the other up to their sums; what is needed again is made again from what was loaded
+    float sums[R][2];
+    auto hidden = [&](int r, int i) {
+      float f[8];
+      if (p.kind == kInt8) decode<kInt8>(codes[r][i], f);
+      else decode<kE4m3>(codes[r][i], f);
+      Eight h = Eight::of(f);
+      // the scale and rstd in one factor: one rounding of their product, a power of two times rstd is exact
+      const Eight s = Eight::all(scale_of(exps[r][i]) * rstd[r]), m = Eight::all(-mean[r] * rstd[r]);
 #pragma unroll
-            for (int j = 0; j < V; ++j) gm[j] = g1[j];
-          } else {
-            load_f32<V>(p.gamma + col, gm);
-          }
+      for (int j = 0; j < 4; ++j) h.p[j] = f2_fma(h.p[j], s.p[j], m.p[j]);
+      return h;
+    };
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            acc_g[i][j] = fmaf(g[j], h[j], acc_g[i][j]);
-            acc_b[i][j] += g[j];
-            const float gh = g[j] * gm[j];
-            s1 += gh;
-            s2 = fmaf(gh, h[j], s2);
+    for (int r = 0; r < R; ++r) {
+      Eight s1 = Eight::all(0.f), s2 = s1;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (at + i * stride) * 8;
+        if (live[r] && col < d) {
+          const Eight h = hidden(r, i), g = Eight::of(gy[r][i]), gm = NV == 1 ? g1 : load_param<ALIGNED>(p.gamma, col, d);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            acc_g[i].p[j] = f2_fma(g.p[j], h.p[j], acc_g[i].p[j]);
+            acc_b[i].p[j] = f2_add(acc_b[i].p[j], g.p[j]);
+            const uint64_t gh = f2_mul(g.p[j], gm.p[j]);
+            s1.p[j] = f2_add(s1.p[j], gh);
+            s2.p[j] = f2_fma(gh, h.p[j], s2.p[j]);
           }
         }
       }
-      team_sum<TPR>(s1, s2, slots, turn);
-      s1 *= inv_d;
-      s2 *= inv_d;
+      sums[r][0] = s1.sum();
+      sums[r][1] = s2.sum();
+    }
+    team_sum<TPR>(reinterpret_cast<float(&)[2 * R]>(sums), slots, turn);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + r * pl.TEAMS + pl.team;
+      // gx = gh rstd - (rstd mean(gh) + h rstd mean(gh h))
+      const Eight k0 = Eight::all(rstd[r]), k1 = Eight::all(-sums[r][0] * inv_d * rstd[r]), k2 = Eight::all(-sums[r][1] * inv_d * rstd[r]);
+      uint32_t last[4] = {};
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int col = (at + i * stride) * V;
-        if (live && col < d) {
-          float h[V], g[V], gm[V], o[V];
-          hidden(i, h);
-          rgy[r][i].get(g);
-          if (NV == 1) {
+        const int col = (at + i * stride) * 8;
+        Raw8<T> out;
+        out.zero();
+        if (live[r] && col < d) {
+          const Eight h = hidden(r, i), g = Eight::of(gy[r][i]), gm = NV == 1 ? g1 : load_param<ALIGNED>(p.gamma, col, d);
+          Eight o;
 #pragma unroll
-            for (int j = 0; j < V; ++j) gm[j] = g1[j];
-          } else {
-            load_f32<V>(p.gamma + col, gm);
-          }
-          if (p.gres) rres[r][i].get(o);
+          for (int j = 0; j < 4; ++j) o.p[j] = f2_fma(h.p[j], k2.p[j], f2_fma(f2_mul(g.p[j], gm.p[j]), k0.p[j], k1.p[j]));
+          if (RES) {
+            const Eight w = Eight::of(r2[r][i]);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float gx = rstd[r] * (fmaf(g[j], gm[j], -s1) - h[j] * s2);
-            o[j] = p.gres ? o[j] + gx : gx;
+            for (int j = 0; j < 4; ++j) o.p[j] = f2_add(o.p[j], w.p[j]);
           }
-          Raw<T, V> out;
-          out.set(o);
-          out.store(p.gx + row * p.ldgx + col);
+          float f[8];
+          o.split(f);
+          out.set(f);
         }
+        store_piece<ALIGNED, TPR>(out, p.gx + row * p.ldgx, at + i * stride, d, live[r], last);
       }
     }
   }
   pdl_trigger();
   float* to_g = p.parts ? p.parts + (int64_t)blockIdx.x * 2 * d : p.g_gamma;
   float* to_b = p.parts ? to_g + d : p.g_beta;
-  if constexpr (TPR <= 0) {
+  float sum_g[NV][8], sum_b[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    acc_g[i].split(sum_g[i]);
+    acc_b[i].split(sum_b[i]);
+  }
+  if constexpr (TPR == 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = (at + i * stride) * V;
+      const int col = (at + i * stride) * 8;
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (col < d) {
-          if (to_g) to_g[col + j] = acc_g[i][j];
-          if (to_b) to_b[col + j] = acc_b[i][j];
+      for (int j = 0; j < 8; ++j)
+        if (col + j < d) {
+          if (to_g) to_g[col + j] = sum_g[i][j];
+          if (to_b) to_b[col + j] = sum_b[i][j];
         }
     }
   } else {
 #pragma unroll
-    for (int o = W; o < 32; o <<= 1)
+    for (int o = pl.TEAM; o < 32; o <<= 1)
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          acc_g[i][j] += __shfl_xor_sync(0xffffffffu, acc_g[i][j], o);
-          acc_b[i][j] += __shfl_xor_sync(0xffffffffu, acc_b[i][j], o);
+        for (int j = 0; j < 8; ++j) {
+          sum_g[i][j] += __shfl_xor_sync(0xffffffffu, sum_g[i][j], o);
+          sum_b[i][j] += __shfl_xor_sync(0xffffffffu, sum_b[i][j], o);
         }
     const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     for (int w = 0; w < warps; ++w) {
-      if (warp == w && team == 0) {
+      if (warp == w && pl.team == 0) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          const int col = (at + i * stride) * V;
-          if (col < d) {
+          const int col = (at + i * stride) * 8;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              s_sums[col + j] = w ? s_sums[col + j] + acc_g[i][j] : acc_g[i][j];
-              s_sums[d + col + j] = w ? s_sums[d + col + j] + acc_b[i][j] : acc_b[i][j];
+          for (int j = 0; j < 8; ++j)
+            if (col + j < d) {
+              s_sums[col + j] = w ? s_sums[col + j] + sum_g[i][j] : sum_g[i][j];
+              s_sums[d + col + j] = w ? s_sums[d + col + j] + sum_b[i][j] : sum_b[i][j];
             }
-          }
         }
       }
       __syncthreads();
@@ -377,91 +462,90 @@ __global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? bwd_resident(NV 
   }
 }
 
-// How rows of d elements are shared out: lanes per team (TPR), steps per lane, rows in flight
+constexpr int rows_together(int nv) { return nv == 1 ? 2 : 1; }
+
+// How rows of d elements are shared out: lanes per team (TPR), steps per lane, rows worked on together
 struct Shape {
-  int v, tpr, nv, r;
+  int tpr, nv, r;
   int threads;             // per block
   int rows_per_block;
   int resident;            // blocks per SM
 };
-constexpr int kMaxWidth = 16384;
-inline Shape shape_of(int d, bool vec, bool bwd) {
-  const int pitch = (int)pitch_of(d);
+constexpr int kMaxWidth = 8192;
+// Rows of 513 to 1,024: the forward of aligned ones by a warp's lanes (65,536 x 1,024 bf16 with a residual 109 us, a block 129), the backward by
+// blocks (118 us; a warp's lanes, with 64 running sums each, 202)
+inline Shape shape_of(int d, bool aligned, bool bwd) {
+  const int pieces = (int)pitch_of(d) / 8;
   Shape s;
-  s.v = vec ? 8 : 1;
-  s.r = 1;
-  if (vec) {
-    const int pieces = pitch / 8;
-    if (pieces <= 128) {
-      s.tpr = pieces <= 4 ? 4 : pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
-      s.nv = pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4;
-      s.r = s.nv == 1 ? 2 : 1;
-    } else {
-      s.nv = 2;
-      s.tpr = pieces <= 1024 ? 0 : -1;
-    }
-  } else if (pitch <= 1024) {
-    s.tpr = 32;
-    s.nv = pitch <= 256 ? 8 : 32;
-  } else {
-    s.nv = 16;
-    s.tpr = pitch <= 8192 ? 0 : -1;
-  }
-  if (s.tpr > 0) {
+  if (pieces <= (bwd || !aligned ? 64 : 128)) {
+    s.tpr = pieces <= 4 ? 4 : pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
+    s.nv = pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4;
+    s.r = rows_together(s.nv);
     s.threads = kThreads;
     s.rows_per_block = kThreads / s.tpr * s.r;
-    s.resident = bwd ? bwd_resident(s.nv * s.v * s.r) : fwd_resident(s.nv * s.v * s.r);
+    s.resident = kResident;
   } else {
-    s.threads = (int)round_up((pitch / s.v + s.nv - 1) / s.nv, 32);
-    s.rows_per_block = 1;
-    s.resident = (bwd ? 1024 : 2048) / s.threads;
+    s.tpr = 0;
+    s.nv = pieces <= 512 ? 1 : 2;
+    s.r = rows_together(s.nv);
+    s.threads = (int)round_up((pieces + s.nv - 1) / s.nv, 32);
+    s.rows_per_block = s.r;
+    s.resident = (bwd ? 512 : 1024) / s.threads;
     if (s.resident < 1) s.resident = 1;
   }
   return s;
 }
-inline int blocks_of(const Shape& s, int64_t rows, int waves) {
-  const int64_t need = (rows + s.rows_per_block - 1) / s.rows_per_block, cap = (int64_t)sm_count() * s.resident * waves;
+inline int blocks_of(const Shape& s, int64_t rows) {
+  const int64_t need = (rows + s.rows_per_block - 1) / s.rows_per_block, cap = (int64_t)sm_count() * s.resident;
   return (int)(need < cap ? need : cap);
 }
 
 template <typename T, typename TY>
-int fwd(const FwdArgs<T, TY>& p, bool vec, cudaStream_t stream);
+int fwd(const FwdArgs<T, TY>& p, bool aligned, cudaStream_t stream);
 template <typename T, typename TY>
-int bwd(const BwdArgs<T, TY>& p, bool vec, cudaStream_t stream);      // p.parts: blocks_of(shape_of(d, vec, true), rows, 1) rows of 2 d floats if that is above 1
+int bwd(const BwdArgs<T, TY>& p, bool aligned, cudaStream_t stream);      // p.parts: blocks_of(shape_of(d, aligned, true), rows) rows of 2 d floats if that is above 1
 
-// calls fn(V, TPR, NV, R as integral constants) for the shape
+// calls fn(TPR, NV, rows together if NV = 1 and a warp's lanes hold the row) for the shape
 template <typename Fn>
 void with_shape(const Shape& s, Fn&& fn) {
-#define BSRL_SHAPE(V_, TPR_, NV_, R_) \
-  if (s.v == V_ && s.tpr == TPR_ && s.nv == NV_) return fn(std::integral_constant<int, V_>{}, std::integral_constant<int, TPR_>{}, std::integral_constant<int, NV_>{}, std::integral_constant<int, R_>{})
-  BSRL_SHAPE(8, 4, 1, 2);
-  BSRL_SHAPE(8, 8, 1, 2);
-  BSRL_SHAPE(8, 16, 1, 2);
-  BSRL_SHAPE(8, 32, 1, 2);
-  BSRL_SHAPE(8, 32, 2, 1);
-  BSRL_SHAPE(8, 32, 4, 1);
-  BSRL_SHAPE(8, 0, 2, 1);
-  BSRL_SHAPE(8, -1, 2, 1);
-  BSRL_SHAPE(1, 32, 8, 1);
-  BSRL_SHAPE(1, 32, 32, 1);
-  BSRL_SHAPE(1, 0, 16, 1);
-  BSRL_SHAPE(1, -1, 16, 1);
+#define BSRL_SHAPE(TPR_, NV_) \
+  if (s.tpr == TPR_ && s.nv == NV_) return fn(std::integral_constant<int, TPR_>{}, std::integral_constant<int, NV_>{})
+  BSRL_SHAPE(4, 1);
+  BSRL_SHAPE(8, 1);
+  BSRL_SHAPE(16, 1);
+  BSRL_SHAPE(32, 1);
+  BSRL_SHAPE(32, 2);
+  BSRL_SHAPE(32, 4);                                 // forward only
+  BSRL_SHAPE(0, 1);
+  BSRL_SHAPE(0, 2);
 #undef BSRL_SHAPE
 }
 template <typename T, typename TY>
-int launch_fwd(const FwdArgs<T, TY>& p, bool vec, cudaStream_t stream) {
-  const Shape s = shape_of(p.d, vec, false);
-  const int blocks = blocks_of(s, p.rows, 4);
-  with_shape(s, [&](auto V, auto TPR, auto NV, auto R) { launch_kernel(norm8_fwd_kernel<T, TY, V(), TPR(), NV(), R()>, blocks, s.threads, 0, stream, p); });
+int launch_fwd(const FwdArgs<T, TY>& p, bool aligned, cudaStream_t stream) {
+  const Shape s = shape_of(p.d, aligned, false);
+  const int blocks = blocks_of(s, p.rows);
+  with_shape(s, [&](auto TPR, auto NV) {
+    constexpr int R = rows_together(NV());
+    if (!aligned) launch_kernel(norm8_fwd_kernel<T, TY, false, true, TPR(), NV(), R>, blocks, s.threads, 0, stream, p);
+    else if (p.res) launch_kernel(norm8_fwd_kernel<T, TY, true, true, TPR(), NV(), R>, blocks, s.threads, 0, stream, p);
+    else launch_kernel(norm8_fwd_kernel<T, TY, true, false, TPR(), NV(), R>, blocks, s.threads, 0, stream, p);
+  });
   BSRL_LAUNCH_OK("norm8_fwd_kernel");
   return BSRL_OK;
 }
 template <typename T, typename TY>
-int launch_bwd(const BwdArgs<T, TY>& p, bool vec, cudaStream_t stream) {
-  const Shape s = shape_of(p.d, vec, true);
-  const int blocks = blocks_of(s, p.rows, 1);
+int launch_bwd(const BwdArgs<T, TY>& p, bool aligned, cudaStream_t stream) {
+  const Shape s = shape_of(p.d, aligned, true);
+  const int blocks = blocks_of(s, p.rows);
   const size_t smem = s.tpr > 0 ? 2 * p.d * sizeof(float) : 0;
-  with_shape(s, [&](auto V, auto TPR, auto NV, auto R) { launch_kernel(norm8_bwd_kernel<T, TY, V(), TPR(), NV(), R()>, blocks, s.threads, smem, stream, p); });
+  with_shape(s, [&](auto TPR, auto NV) {
+    constexpr int R = rows_together(NV());
+    if constexpr (NV() <= 2) {
+    if (!aligned) launch_kernel(norm8_bwd_kernel<T, TY, false, true, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
+    else if (p.gres) launch_kernel(norm8_bwd_kernel<T, TY, true, true, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
+    else launch_kernel(norm8_bwd_kernel<T, TY, true, false, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
+    }
+  });
   BSRL_LAUNCH_OK("norm8_bwd_kernel");
   return BSRL_OK;
 }

@@ -4,32 +4,32 @@
 namespace bsrl {
 namespace norm8 {
 template <>
-int fwd(const FwdArgs<__half, __half>& p, bool vec, cudaStream_t stream) { return launch_fwd(p, vec, stream); }
+int fwd(const FwdArgs<__half, __half>& p, bool aligned, cudaStream_t stream) { return launch_fwd(p, aligned, stream); }
 template <>
-int fwd(const FwdArgs<__nv_bfloat16, __nv_bfloat16>& p, bool vec, cudaStream_t stream) { return launch_fwd(p, vec, stream); }
+int fwd(const FwdArgs<__nv_bfloat16, __nv_bfloat16>& p, bool aligned, cudaStream_t stream) { return launch_fwd(p, aligned, stream); }
 template <>
-int bwd(const BwdArgs<__half, __half>& p, bool vec, cudaStream_t stream) { return launch_bwd(p, vec, stream); }
+int bwd(const BwdArgs<__half, __half>& p, bool aligned, cudaStream_t stream) { return launch_bwd(p, aligned, stream); }
 template <>
-int bwd(const BwdArgs<__nv_bfloat16, __nv_bfloat16>& p, bool vec, cudaStream_t stream) { return launch_bwd(p, vec, stream); }
+int bwd(const BwdArgs<__nv_bfloat16, __nv_bfloat16>& p, bool aligned, cudaStream_t stream) { return launch_bwd(p, aligned, stream); }
 
 namespace {
-// out = sum over parts (n_parts, cols), in order: a block takes 32 columns, its 8 warps every eighth part each, then the warps' sums one
+// out = sum over parts (n_parts, cols), in order: a block takes 32 columns, its 32 warps every 32nd part each, then the warps' sums one
 // after the other.  The first d columns go to a, the others to b.
-__global__ void __launch_bounds__(256) add_parts_kernel(const float* __restrict__ parts, int n_parts, int d, float* a, float* b) {
+__global__ void __launch_bounds__(1024) add_parts_kernel(const float* __restrict__ parts, int n_parts, int d, float* a, float* b) {
   pdl_begin();
-  __shared__ float s[8][33];
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + lane, cols = 2 * d;
   float sum = 0.f;
   if (col < cols) {
 #pragma unroll 8
-    for (int p = warp; p < n_parts; p += 8) sum += parts[(int64_t)p * cols + col];
+    for (int p = warp; p < n_parts; p += 32) sum += parts[(int64_t)p * cols + col];
   }
   s[warp][lane] = sum;
   __syncthreads();
   if (warp == 0 && col < cols) {
 #pragma unroll
-    for (int w = 1; w < 8; ++w) sum += s[w][lane];
+    for (int w = 1; w < 32; ++w) sum += s[w][lane];
     if (col < d) {
       if (a) a[col] = sum;
     } else if (b) {
@@ -58,18 +58,18 @@ template <typename T, typename TY>
 int run_fwd(const Norm8Args& a, cudaStream_t stream) {
   const FwdArgs<T, TY> p{static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<T*>(a.z), static_cast<TY*>(a.y), a.gamma, a.beta,
                          a.codes, a.exps, a.mean, a.rstd, a.rows, a.ldx, a.ldr, a.ldz, a.ldy, a.d, a.kind, a.eps};
-  const bool vec = by16(a.d, {{a.x, a.ldx, sizeof(T)}, {a.residual, a.ldr, sizeof(T)}, {a.z, a.ldz, sizeof(T)}, {a.y, a.ldy, sizeof(TY)}, {a.gamma, 4, 4}, {a.beta, 4, 4}});
-  return fwd<T, TY>(p, vec, stream);
+  const bool aligned = by16(a.d, {{a.x, a.ldx, sizeof(T)}, {a.residual, a.ldr, sizeof(T)}, {a.z, a.ldz, sizeof(T)}, {a.y, a.ldy, sizeof(TY)}, {a.gamma, 4, 4}, {a.beta, 4, 4}});
+  return fwd<T, TY>(p, aligned, stream);
 }
 bool bwd_by16(const Norm8BwdArgs& a) {
   const int t = a.dtype == BSRL_F32 ? 4 : 2, ty = a.gy_dtype == BSRL_F32 ? 4 : 2;
   return by16(a.d, {{a.gy, a.ldgy, ty}, {a.g_residual, a.ldgr, t}, {a.gx, a.ldgx, t}, {a.gamma, 4, 4}});
 }
 template <typename T, typename TY>
-int run_bwd(const Norm8BwdArgs& a, bool vec, float* parts, cudaStream_t stream) {
+int run_bwd(const Norm8BwdArgs& a, bool aligned, float* parts, cudaStream_t stream) {
   const BwdArgs<T, TY> p{static_cast<const TY*>(a.gy), static_cast<const T*>(a.g_residual), static_cast<T*>(a.gx), a.gamma, a.codes, a.exps,
                          a.mean, a.rstd, a.g_gamma, a.g_beta, parts, a.rows, a.ldgy, a.ldgr, a.ldgx, a.d, a.kind};
-  return bwd<T, TY>(p, vec, stream);
+  return bwd<T, TY>(p, aligned, stream);
 }
 }  // namespace
 
@@ -87,29 +87,24 @@ int norm8_fwd(const Norm8Args& a, cudaStream_t stream) {
   return run_fwd<float, float>(a, stream);
 }
 
-// Enough for either way of sharing out the rows, so that the size does not depend on pointers.
 int64_t norm8_bwd_workspace(int64_t rows, int d) {
-  int most = 0;
-  for (bool vec : {false, true}) {
-    const int n = blocks_of(shape_of(d, vec, true), rows, 1);
-    if (n > most) most = n;
-  }
-  return most > 1 ? (int64_t)most * 2 * d * (int64_t)sizeof(float) : 0;
+  const int blocks = blocks_of(shape_of(d, true, true), rows);            // the backward shares out both kinds of rows alike
+  return blocks > 1 ? (int64_t)blocks * 2 * d * (int64_t)sizeof(float) : 0;
 }
 int norm8_bwd(const Norm8BwdArgs& a, float* workspace, cudaStream_t stream) {
-  const bool vec = bwd_by16(a);
-  const int blocks = blocks_of(shape_of(a.d, vec, true), a.rows, 1);
+  const bool aligned = bwd_by16(a);
+  const int blocks = blocks_of(shape_of(a.d, aligned, true), a.rows);
   float* parts = blocks > 1 && (a.g_gamma || a.g_beta) ? workspace : nullptr;
   int rc;
-  if (a.dtype == BSRL_F16) rc = run_bwd<__half, __half>(a, vec, parts, stream);
-  else if (a.dtype == BSRL_BF16) rc = run_bwd<__nv_bfloat16, __nv_bfloat16>(a, vec, parts, stream);
-  else if (a.gy_dtype == BSRL_F16) rc = run_bwd<float, __half>(a, vec, parts, stream);
-  else if (a.gy_dtype == BSRL_BF16) rc = run_bwd<float, __nv_bfloat16>(a, vec, parts, stream);
-  else rc = run_bwd<float, float>(a, vec, parts, stream);
+  if (a.dtype == BSRL_F16) rc = run_bwd<__half, __half>(a, aligned, parts, stream);
+  else if (a.dtype == BSRL_BF16) rc = run_bwd<__nv_bfloat16, __nv_bfloat16>(a, aligned, parts, stream);
+  else if (a.gy_dtype == BSRL_F16) rc = run_bwd<float, __half>(a, aligned, parts, stream);
+  else if (a.gy_dtype == BSRL_BF16) rc = run_bwd<float, __nv_bfloat16>(a, aligned, parts, stream);
+  else rc = run_bwd<float, float>(a, aligned, parts, stream);
   if (rc != BSRL_OK || !parts) return rc;
   PdlScope overlap;
   pdl_enable();
-  launch_kernel(add_parts_kernel, (unsigned)((2 * a.d + 31) / 32), 256, 0, stream, static_cast<const float*>(parts), blocks, a.d, a.g_gamma, a.g_beta);
+  launch_kernel(add_parts_kernel, (unsigned)((2 * a.d + 31) / 32), 1024, 0, stream, static_cast<const float*>(parts), blocks, a.d, a.g_gamma, a.g_beta);
   BSRL_LAUNCH_OK("add_parts_kernel");
   return BSRL_OK;
 }

@@ -4,16 +4,16 @@
 namespace bsrl {
 namespace norm8 {
 template <>
-int fwd(const FwdArgs<float, float>& p, bool vec, cudaStream_t stream) { return launch_fwd(p, vec, stream); }
+int fwd(const FwdArgs<float, float>& p, bool aligned, cudaStream_t stream) { return launch_fwd(p, aligned, stream); }
 template <>
-int fwd(const FwdArgs<float, __half>& p, bool vec, cudaStream_t stream) { return launch_fwd(p, vec, stream); }
+int fwd(const FwdArgs<float, __half>& p, bool aligned, cudaStream_t stream) { return launch_fwd(p, aligned, stream); }
 template <>
-int fwd(const FwdArgs<float, __nv_bfloat16>& p, bool vec, cudaStream_t stream) { return launch_fwd(p, vec, stream); }
+int fwd(const FwdArgs<float, __nv_bfloat16>& p, bool aligned, cudaStream_t stream) { return launch_fwd(p, aligned, stream); }
 template <>
-int bwd(const BwdArgs<float, float>& p, bool vec, cudaStream_t stream) { return launch_bwd(p, vec, stream); }
+int bwd(const BwdArgs<float, float>& p, bool aligned, cudaStream_t stream) { return launch_bwd(p, aligned, stream); }
 template <>
-int bwd(const BwdArgs<float, __half>& p, bool vec, cudaStream_t stream) { return launch_bwd(p, vec, stream); }
+int bwd(const BwdArgs<float, __half>& p, bool aligned, cudaStream_t stream) { return launch_bwd(p, aligned, stream); }
 template <>
-int bwd(const BwdArgs<float, __nv_bfloat16>& p, bool vec, cudaStream_t stream) { return launch_bwd(p, vec, stream); }
+int bwd(const BwdArgs<float, __nv_bfloat16>& p, bool aligned, cudaStream_t stream) { return launch_bwd(p, aligned, stream); }
 }  // namespace norm8
 }  // namespace bsrl

@@ -22,24 +22,7 @@ enum Kind { kInt8 = 0, kE4m3 = 1 };
 
 __host__ __device__ __forceinline__ int64_t pitch_of(int64_t d) { return (d + kBlock - 1) / kBlock * kBlock; }
 
-// ---- loads and stores of V neighbouring elements (V = 8: 16-byte aligned; V = 1: any)
-template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
+// ---- eight neighbouring elements of a row
 // two 16-bit elements of a word <-> two floats
 template <typename T>
 __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b);
@@ -64,68 +47,176 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// V elements as they lie in memory: few registers between the request and the use
-template <typename T, int V>
-struct Raw {
-  T v[V];
-  __device__ __forceinline__ void load(const T* p) { v[0] = *p; }
-  __device__ __forceinline__ void zero() { v[0] = from_f32<T>(0.f); }
-  __device__ __forceinline__ void get(float (&f)[V]) const { f[0] = to_f32(v[0]); }
-  __device__ __forceinline__ void set(const float (&f)[V]) { v[0] = from_f32<T>(f[0]); }
-  __device__ __forceinline__ void store(T* p) const { *p = v[0]; }
-};
-template <>
-struct Raw<float, 8> {
-  float4 v[2];
-  __device__ __forceinline__ void load(const float* p) {
-    v[0] = reinterpret_cast<const float4*>(p)[0];
-    v[1] = reinterpret_cast<const float4*>(p)[1];
+// as they lie in memory: few registers between the request and the use
+template <typename T>
+struct Raw8 {                                    // 16 bits
+  static constexpr int kWords = 4;
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   }
-  __device__ __forceinline__ void zero() { v[0] = v[1] = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
+  __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0; }
   __device__ __forceinline__ void get(float (&f)[8]) const {
-    f[0] = v[0].x; f[1] = v[0].y; f[2] = v[0].z; f[3] = v[0].w;
-    f[4] = v[1].x; f[5] = v[1].y; f[6] = v[1].z; f[7] = v[1].w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) unpack2<T>(w[j], f[2 * j], f[2 * j + 1]);
   }
   __device__ __forceinline__ void set(const float (&f)[8]) {
-    v[0] = make_float4(f[0], f[1], f[2], f[3]);
-    v[1] = make_float4(f[4], f[5], f[6], f[7]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = pack2<T>(f[2 * j], f[2 * j + 1]);
+  }
+  __device__ __forceinline__ void load1(const T* p, int e) {       // element e, the others of its word kept
+    const uint32_t v = *reinterpret_cast<const uint16_t*>(p + e);
+    w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | v << 16 : (w[e >> 1] & 0xffff0000u) | v;
+  }
+  __device__ __forceinline__ void store1(T* p, int e) const { *reinterpret_cast<uint16_t*>(p + e) = (uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]); }
+};
+template <>
+struct Raw8<float> {
+  static constexpr int kWords = 8;
+  uint32_t w[8];
+  __device__ __forceinline__ void load(const float* p) {
+    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
   }
   __device__ __forceinline__ void store(float* p) const {
-    reinterpret_cast<float4*>(p)[0] = v[0];
-    reinterpret_cast<float4*>(p)[1] = v[1];
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
-};
-template <typename T>
-struct Raw16x8 {
-  uint4 v;
-  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = 0;
+  }
   __device__ __forceinline__ void get(float (&f)[8]) const {
-    unpack2<T>(v.x, f[0], f[1]);
-    unpack2<T>(v.y, f[2], f[3]);
-    unpack2<T>(v.z, f[4], f[5]);
-    unpack2<T>(v.w, f[6], f[7]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
   }
   __device__ __forceinline__ void set(const float (&f)[8]) {
-    v = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(f[j]);
   }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = v; }
+  __device__ __forceinline__ void load1(const float* p, int e) { w[e] = *reinterpret_cast<const uint32_t*>(p + e); }
+  __device__ __forceinline__ void store1(float* p, int e) const { *reinterpret_cast<uint32_t*>(p + e) = w[e]; }
 };
-template <>
-struct Raw<__half, 8> : Raw16x8<__half> {};
-template <>
-struct Raw<__nv_bfloat16, 8> : Raw16x8<__nv_bfloat16> {};
 
-// V codes
-template <int V>
-struct Codes {
-  uint8_t v;
-  __device__ __forceinline__ void load(const uint8_t* p) { v = *p; }
-  __device__ __forceinline__ void store(uint8_t* p) const { *p = v; }
-  __device__ __forceinline__ void zero() { v = 0; }
+// eight numbers as four pairs: two fp32 operations per instruction
+struct Eight {
+  uint64_t p[4];
+  template <typename T>
+  __device__ __forceinline__ static Eight of(const Raw8<T>& r) {
+    float f[8];
+    r.get(f);
+    return of(f);
+  }
+  __device__ __forceinline__ static Eight of(const float (&f)[8]) {
+    Eight e;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e.p[i] = f2_make(f[2 * i], f[2 * i + 1]);
+    return e;
+  }
+  __device__ __forceinline__ static Eight all(float v) {
+    Eight e;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e.p[i] = f2_make(v, v);
+    return e;
+  }
+  __device__ __forceinline__ void split(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f2_split(p[i], f[2 * i], f[2 * i + 1]);
+  }
+  __device__ __forceinline__ float sum() const {
+    float a, b;
+    f2_split(f2_add(f2_add(p[0], p[1]), f2_add(p[2], p[3])), a, b);
+    return a + b;
+  }
 };
-template <>
-struct Codes<8> {
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Where a matrix's bytes begin and end: pieces that do not start on 16 bytes are read by the aligned 16 bytes around them, inside these
+struct Span {
+  const uint8_t* lo;
+  const uint8_t* hi;
+};
+template <typename T>
+__host__ __device__ __forceinline__ Span span_of(const T* p, int64_t rows, int64_t d, int64_t ld) {
+  return Span{reinterpret_cast<const uint8_t*>(p), reinterpret_cast<const uint8_t*>(p + (rows - 1) * ld + d)};
+}
+
+// N 32-bit words from byte `by` (0 .. 15, a multiple of the element's size) of the words c
+template <int N, bool HALVES, int M>
+__device__ __forceinline__ void take_words(uint32_t (&c)[M], int by, uint32_t* out) {
+  static_assert(M >= N + 4, "");
+  const int k = by >> 2;
+#pragma unroll
+  for (int j = 0; j + 1 < M; ++j) c[j] = k & 1 ? c[j + 1] : c[j];
+#pragma unroll
+  for (int j = 0; j + 2 < M; ++j) c[j] = k & 2 ? c[j + 2] : c[j];
+#pragma unroll
+  for (int j = 0; j < N; ++j) out[j] = HALVES ? __funnelshift_r(c[j], c[j + 1], (by & 2) * 8) : c[j];
+}
+// A piece anywhere in memory, of which `n` elements exist (the others read as zero)
+template <typename T>
+__device__ __forceinline__ void load_any(Raw8<T>& r, const T* p, int n, const Span& s) {
+  constexpr int W = Raw8<T>::kWords;
+  const int by = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+  const uint8_t* from = reinterpret_cast<const uint8_t*>(p) - by;
+  if (n >= 8 && by == 0) {
+    r.load(p);
+  } else if (n >= 8 && from >= s.lo && from + W * 4 + 16 <= s.hi) {
+    uint32_t c[W + 4];
+#pragma unroll
+    for (int j = 0; j < W + 4; j += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(from + j * 4);
+      c[j] = v.x; c[j + 1] = v.y; c[j + 2] = v.z; c[j + 3] = v.w;
+    }
+    take_words<W, W == 4>(c, by, r.w);
+  } else {
+    r.zero();
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) r.load1(p, e);
+  }
+}
+// The same the other way.  The aligned 16 bytes that two neighbouring pieces share are written by the later one: `prev` holds the last
+// 16 bytes of the piece ahead where that is whole and in this call (`ahead`); `behind`: the next one is whole and takes this one's end.
+template <typename T>
+__device__ __forceinline__ void store_any(const Raw8<T>& r, T* p, int n, const uint32_t (&prev)[4], bool ahead, bool behind) {
+  constexpr int W = Raw8<T>::kWords, SIZE = (int)sizeof(T);
+  const int by = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+  if (n >= 8 && by == 0) {
+    r.store(p);
+    return;
+  }
+  int head = 0, tail = 8;                          // elements below head and from tail on go one by one
+  if (n >= 8) {
+    uint32_t c[W + 4], o[W];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = prev[j];
+#pragma unroll
+    for (int j = 0; j < W; ++j) c[4 + j] = r.w[j];
+    take_words<W, W == 4>(c, 16 - by, o);
+    uint8_t* to = reinterpret_cast<uint8_t*>(p) - by;
+    if (ahead) *reinterpret_cast<uint4*>(to) = make_uint4(o[0], o[1], o[2], o[3]);
+    else head = (16 - by) / SIZE;
+    if constexpr (W == 8) *reinterpret_cast<uint4*>(to + 16) = make_uint4(o[4], o[5], o[6], o[7]);
+    if (!behind) tail = 8 - by / SIZE;
+  } else {
+    head = n;
+  }
+  if (head > 0 || tail < 8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < head || e >= tail) r.store1(p, e);
+  }
+}
+
+// eight codes
+struct Codes {
   uint2 v;
   __device__ __forceinline__ void load(const uint8_t* p) { v = *reinterpret_cast<const uint2*>(p); }
   __device__ __forceinline__ void store(uint8_t* p) const { *reinterpret_cast<uint2*>(p) = v; }
@@ -138,19 +229,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {      // NaN wins
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// largest magnitude (its bits; NaN above all) of the block whose values the V-wide lanes of a group hold
-template <int V>
-__device__ __forceinline__ uint32_t block_max_bits(const float (&f)[V]) {
-  if constexpr (V == 1) {
-    return __reduce_max_sync(0xffffffffu, __float_as_uint(f[0]) & 0x7fffffffu);
-  } else {
-    float m = fabsf(f[0]);
-#pragma unroll
-    for (int i = 1; i < V; ++i) m = max_nan(m, fabsf(f[i]));
-    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    return __float_as_uint(m) & 0x7fffffffu;
-  }
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// largest magnitude (its bits; NaN above all) of the block that four lanes hold
+__device__ __forceinline__ uint32_t block_max_bits(const float (&f)[8]) {
+  float m = max_abs(max_abs(max_abs(f[0], f[1], f[2]), f[3], f[4]), max_abs(f[5], f[6], f[7]), 0.f);
+  m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  return __float_as_uint(m) & 0x7fffffffu;
 }
 
 // Per kind: log2 of the range's top binade, and what is added to the largest magnitude's bits so that a mantissa whose code would
@@ -169,8 +258,8 @@ __device__ constexpr int top_binade<__half>() { return 15; }
 
 // E of a block, the factor that takes its values to codes, and -- in the top binade only, or where something is not finite -- the
 // values themselves brought into the range.
-template <typename T, int KIND, int V>
-__device__ __forceinline__ uint32_t block_exp(uint32_t bits, float (&f)[V], float& inv) {
+template <typename T, int KIND>
+__device__ __forceinline__ uint32_t block_exp(uint32_t bits, float (&f)[8], float& inv) {
   using K = KindOf<KIND>;
   constexpr uint32_t kPast = (uint32_t)(top_binade<T>() + 128) << 23;                // 2^(top + 1); fp32: infinity
   uint32_t e = (bits + K::kCarry) >> 23;
@@ -178,12 +267,12 @@ __device__ __forceinline__ uint32_t block_exp(uint32_t bits, float (&f)[V], floa
     if (bits >= 0x7f800000u) {
       inv = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = 0.f;
+      for (int i = 0; i < 8; ++i) f[i] = 0.f;
       return 255;
     }
     constexpr float kMost = K::kTop * (top_binade<T>() == 15 ? 32768.f : 1.7014118346046923e38f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = fminf(fmaxf(f[i], -kMost), kMost);
+    for (int i = 0; i < 8; ++i) f[i] = fminf(fmaxf(f[i], -kMost), kMost);
     e = bits >> 23;
   }
   e = e > K::kUp ? e - K::kUp : 0;
@@ -211,13 +300,9 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, 
   }
 }
 template <int KIND>
-__device__ __forceinline__ void encode(const float (&f)[8], float inv, Codes<8>& c) {
+__device__ __forceinline__ void encode(const float (&f)[8], float inv, Codes& c) {
   c.v.x = encode4<KIND>(f[0], f[1], f[2], f[3], inv);
   c.v.y = encode4<KIND>(f[4], f[5], f[6], f[7], inv);
-}
-template <int KIND>
-__device__ __forceinline__ void encode(const float (&f)[1], float inv, Codes<1>& c) {
-  c.v = (uint8_t)encode4<KIND>(f[0], 0.f, 0.f, 0.f, inv);
 }
 
 // codes as numbers, without the scale
@@ -242,14 +327,9 @@ __device__ __forceinline__ void decode4(uint32_t w, float& a, float& b, float& c
   }
 }
 template <int KIND>
-__device__ __forceinline__ void decode(const Codes<8>& c, float (&f)[8]) {
+__device__ __forceinline__ void decode(const Codes& c, float (&f)[8]) {
   decode4<KIND>(c.v.x, f[0], f[1], f[2], f[3]);
   decode4<KIND>(c.v.y, f[4], f[5], f[6], f[7]);
-}
-template <int KIND>
-__device__ __forceinline__ void decode(const Codes<1>& c, float (&f)[1]) {
-  float x, y, z;
-  decode4<KIND>(c.v, f[0], x, y, z);
 }
 // 2^(E - 127); E = 0: 0, E = 255: infinity
 __device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e << 23); }

@@ -283,7 +283,7 @@ int bsrl_linear_bwd(const void* g_f16, const void* x_f16, const void* w_f16, int
  * saved activations shrink to 33/64 (of 16-bit ones) or 33/128.
  *
  * A checkpoint of a (rows, d) matrix is two arrays without gaps: codes (rows, bsrl_pack8_pitch(d)) u8, 16-byte
- * aligned, and exps (rows, bsrl_pack8_pitch(d) / 32) u8.  Blocks of 32 neighbouring values of a row (the last one of a row may be
+ * aligned, and exps (rows, bsrl_pack8_pitch(d) / 32) u8, 4-byte aligned.  Blocks of 32 neighbouring values of a row (the last one of a row may be
  * shorter; its codes end in zeros) share an exponent: value = code 2^(exp - 127), the code being
  *   BSRL_INT8  an int8 in [-127, 127]:          off by at most 1/127 of the block's largest magnitude,
  *   BSRL_E4M3  an e4m3 number in [-240, 240]:   off by at most 2^-4 of the value itself, or 2^-16 of the block's largest.
@@ -294,7 +294,7 @@ int bsrl_linear_bwd(const void* g_f16, const void* x_f16, const void* w_f16, int
  *
  * Matrices have elements of BSRL_F32, BSRL_F16 or BSRL_BF16, rows `ld` elements apart (ld >= d) and no alignment but
  * their elements'; rows that start on 16 bytes, with d a multiple of 8, are faster.  rows may be 0.  d up to 2^31 - 64
- * (bsrl_layernorm8: 16,384).  gamma, beta, mean, rstd and parameter gradients are fp32.  Sums are in fp32 and in one
+ * (bsrl_layernorm8: 8,192).  gamma, beta, mean, rstd and parameter gradients are fp32.  Sums are in fp32 and in one
  * order: a call on the same inputs gives the same bits.  Nothing may overlap except where said. */
 typedef enum bsrl_kind8 { BSRL_INT8 = 0, BSRL_E4M3 = 1 } bsrl_kind8;
 
