@@ -14,6 +14,7 @@ calls can be captured.  Gradients of parameters are fp32 sums in one order: the 
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -76,15 +77,32 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _stream(dev) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+def _call(fn, dev, *args) -> None:
+    """fn(*args, stream) on the device's current stream.  The device is switched only where it is not the current one: with the context
+    manager and a Stream object around every call the small ones took half as long again."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        nat.check(rc)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(fn: str, index: int, *args) -> int:
+    with torch.cuda.device(index):           # what a kernel needs goes by the device's number of SMs
+        n = getattr(nat.lib, fn)(*args)
+    if n < 0:
+        raise nat.BsrlError(int(n), nat.last_error())
+    return n
 
 
 class Checkpoint8:
     """An activation in 8 bits: ``codes`` (rows, pitch) and ``exps`` (rows, pitch / 32), uint8 without gaps, the pitch being the last dimension
     rounded up to 32; ``shape`` and ``dtype`` are those of the activation."""
 
-    __slots__ = ("codes", "exps", "kind", "shape", "dtype")
+    __slots__ = ("kind", "shape", "dtype", "device", "_memory", "_rows", "_blocks", "_codes_ptr", "_exps_ptr")
 
     def __init__(self, codes: torch.Tensor, exps: torch.Tensor, kind: str, shape, dtype: torch.dtype):
         _kind(kind)
@@ -98,39 +116,48 @@ class Checkpoint8:
             rows *= n
         blocks = -(-shape[-1] // BLOCK)
         for t, cols, what in ((codes, blocks * BLOCK, "codes"), (exps, blocks, "exps")):
-            if t.dtype != torch.uint8 or tuple(t.shape) != (rows, cols) or not t.is_contiguous():
+            if t.dtype != torch.uint8 or t.shape != (rows, cols) or not t.is_contiguous():
                 raise ValueError(f"{what} must be contiguous ({rows}, {cols}) uint8, got {tuple(t.shape)} {t.dtype}")
         if codes.device != exps.device:
             raise ValueError(f"codes and exps must be on one device, got {codes.device} and {exps.device}")
-        self.codes, self.exps, self.kind, self.shape, self.dtype = codes, exps, kind, shape, dtype
+        if not codes.is_cuda:
+            raise RuntimeError("a Checkpoint8 must live on a CUDA device (this library has no CPU path)")
+        self.kind, self.shape, self.dtype, self.device = kind, shape, dtype, codes.device
+        self._memory, self._rows, self._blocks = (codes, exps), rows, blocks
+        self._codes_ptr, self._exps_ptr = codes.data_ptr(), exps.data_ptr()
 
     @classmethod
-    def _empty(cls, rows: int, shape, dtype, kind: str, dev) -> "Checkpoint8":
+    def _empty(cls, rows: int, x: torch.Tensor, kind: str) -> "Checkpoint8":
+        """One for x (rows, d), in one piece of memory."""
         self = cls.__new__(cls)
-        blocks = -(-shape[-1] // BLOCK)
-        self.codes = torch.empty(rows, blocks * BLOCK, dtype=torch.uint8, device=dev)
-        self.exps = torch.empty(rows, blocks, dtype=torch.uint8, device=dev)
-        self.kind, self.shape, self.dtype = kind, tuple(shape), dtype
+        blocks = -(-x.shape[-1] // BLOCK)
+        memory = torch.empty(rows * blocks * (BLOCK + 1), dtype=torch.uint8, device=x.device)
+        self.kind, self.shape, self.dtype, self.device = kind, tuple(x.shape), x.dtype, x.device
+        self._memory, self._rows, self._blocks = memory, rows, blocks
+        self._codes_ptr = memory.data_ptr()
+        self._exps_ptr = self._codes_ptr + rows * blocks * BLOCK
         return self
 
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self) -> torch.Tensor:
+        m = self._memory
+        return m[0] if type(m) is tuple else m[:self._rows * self._blocks * BLOCK].view(self._rows, self._blocks * BLOCK)
+
+    @property
+    def exps(self) -> torch.Tensor:
+        m = self._memory
+        return m[1] if type(m) is tuple else m[self._rows * self._blocks * BLOCK:].view(self._rows, self._blocks)
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.exps.numel()
+        return self._rows * self._blocks * (BLOCK + 1)
 
     def expand(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """The values it stands for, in ``dtype`` (default: the activation's)."""
         out = torch.empty(self.shape, dtype=dtype or self.dtype, device=self.device)
-        code = _dtype(out, "dtype")
-        rows, d = self.codes.shape[0], self.shape[-1]
-        if not out.is_cuda:
-            raise RuntimeError("a Checkpoint8 must live on a CUDA device (this library has no CPU path)")
-        with torch.cuda.device(out.device):
-            nat.check(nat.lib.bsrl_expand8(self.codes.data_ptr(), self.exps.data_ptr(), KINDS[self.kind], rows, d, out.data_ptr(), code, d,
-                                           _stream(out.device)))
+        d = self.shape[-1]
+        _call(nat.lib.bsrl_expand8, self.device, self._codes_ptr, self._exps_ptr, KINDS[self.kind], self._rows, d, out.data_ptr(),
+              _dtype(out, "dtype"), d)
         return out
 
 
@@ -138,9 +165,8 @@ def pack8(x: torch.Tensor, kind: str = "int8") -> Checkpoint8:
     """x (..., d) in 8 bits.  Rows may be strided (a slice of wider rows); other strides are copied first."""
     code, k = _dtype(x, "x"), _kind(kind)
     m, rows, d, ld = _rows(x, "x")
-    kept = Checkpoint8._empty(rows, x.shape, x.dtype, kind, x.device)
-    with torch.cuda.device(x.device):
-        nat.check(nat.lib.bsrl_pack8(m.data_ptr(), code, ld, rows, d, k, kept.codes.data_ptr(), kept.exps.data_ptr(), _stream(x.device)))
+    kept = Checkpoint8._empty(rows, x, kind)
+    _call(nat.lib.bsrl_pack8, x.device, m.data_ptr(), code, ld, rows, d, k, kept._codes_ptr, kept._exps_ptr)
     return kept
 
 
@@ -150,22 +176,19 @@ def gelu8_forward(x: torch.Tensor, kind: str = "int8"):
     code, k = _dtype(x, "x"), _kind(kind)
     m, rows, d, ld = _rows(x, "x")
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    kept = Checkpoint8._empty(rows, x.shape, x.dtype, kind, x.device)
-    with torch.cuda.device(x.device):
-        nat.check(nat.lib.bsrl_gelu8(m.data_ptr(), code, ld, rows, d, y.data_ptr(), d, k, kept.codes.data_ptr(), kept.exps.data_ptr(),
-                                     _stream(x.device)))
+    kept = Checkpoint8._empty(rows, x, kind)
+    _call(nat.lib.bsrl_gelu8, x.device, m.data_ptr(), code, ld, rows, d, y.data_ptr(), d, k, kept._codes_ptr, kept._exps_ptr)
     return y, kept
 
 
 def gelu8_backward(gy: torch.Tensor, kept: Checkpoint8) -> torch.Tensor:
     """gy gelu'(x8), in the activation's type."""
-    if tuple(gy.shape) != kept.shape or gy.dtype != kept.dtype or gy.device != kept.device:
+    if gy.shape != kept.shape or gy.dtype != kept.dtype or gy.device != kept.device:
         raise ValueError(f"gy must be {kept.shape} {kept.dtype} on {kept.device}, got {tuple(gy.shape)} {gy.dtype} on {gy.device}")
     m, rows, d, ld = _rows(gy, "gy")
     gx = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device)
-    with torch.cuda.device(gy.device):
-        nat.check(nat.lib.bsrl_gelu8_bwd(m.data_ptr(), _DTYPES[gy.dtype], ld, kept.codes.data_ptr(), kept.exps.data_ptr(), KINDS[kept.kind], rows, d,
-                                         gx.data_ptr(), d, _stream(gy.device)))
+    _call(nat.lib.bsrl_gelu8_bwd, gy.device, m.data_ptr(), _DTYPES[gy.dtype], ld, kept._codes_ptr, kept._exps_ptr, KINDS[kept.kind], rows, d,
+          gx.data_ptr(), d)
     return gx
 
 
@@ -190,10 +213,10 @@ def gelu8(x: torch.Tensor, kind: str = "int8") -> torch.Tensor:
 
 # ------------------------------------------------------------------ LayerNorm
 class LayerNorm8Saved(NamedTuple):
-    """What ``layer_norm8_backward`` needs: the normalised tensor in 8 bits, its rows' mean and 1 / sqrt(var + eps)."""
+    """What ``layer_norm8_backward`` needs: the normalised tensor in 8 bits and ``stats`` (2, rows) fp32, its rows' mean and
+    1 / sqrt(var + eps)."""
     kept: Checkpoint8
-    mean: torch.Tensor
-    rstd: torch.Tensor
+    stats: torch.Tensor
 
 
 def layer_norm8_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
@@ -211,42 +234,38 @@ def layer_norm8_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[to
     if residual is not None:
         res, _, _, ldr = _rows(_same(residual, x, "residual"), "residual")
         z = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    kept = Checkpoint8._empty(rows, x.shape, x.dtype, kind, dev)
-    mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=dev).unbind(0)
-    with torch.cuda.device(dev):
-        nat.check(nat.lib.bsrl_layernorm8(
-            m.data_ptr(), _ptr(res), code, ld, ldr, weight.data_ptr(), _ptr(bias), eps, rows, d, z.data_ptr(), d, y.data_ptr(),
-            _dtype(y, "out_dtype"), d, k, kept.codes.data_ptr(), kept.exps.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _stream(dev)))
-    return y, z, LayerNorm8Saved(kept, mean, rstd)
+    kept = Checkpoint8._empty(rows, x, kind)
+    stats = torch.empty(2, rows, dtype=torch.float32, device=dev)
+    at = stats.data_ptr()
+    _call(nat.lib.bsrl_layernorm8, dev, m.data_ptr(), _ptr(res), code, ld, ldr, weight.data_ptr(), _ptr(bias), eps, rows, d, z.data_ptr(), d,
+          y.data_ptr(), _dtype(y, "out_dtype"), d, k, kept._codes_ptr, kept._exps_ptr, at, at + 4 * rows)
+    return y, z, LayerNorm8Saved(kept, stats)
 
 
 def layer_norm8_backward(gy: torch.Tensor, saved: LayerNorm8Saved, weight: torch.Tensor, g_residual: Optional[torch.Tensor] = None,
                          param_grads: bool = True):
     """(gx, g_weight, g_bias): gx is the gradient of x and of the residual, ``g_residual`` (the gradient that reaches z by other ways)
     added; the parameters' are fp32 and None without ``param_grads``."""
-    kept, mean, rstd = saved
+    kept, stats = saved
     dev = kept.device
-    if tuple(gy.shape) != kept.shape or gy.device != dev:
+    if gy.shape != kept.shape or gy.device != dev:
         raise ValueError(f"gy must be {kept.shape} on {dev}, got {tuple(gy.shape)} on {gy.device}")
     code = _dtype(gy, "gy")
     m, rows, d, ld = _rows(gy, "gy")
     weight = _vector(weight, d, dev, "weight")
-    for t, what in ((mean, "mean"), (rstd, "rstd")):
-        if tuple(t.shape) != (rows,) or t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{what} must be contiguous ({rows},) float32 on {dev}")
+    if stats.shape != (2, rows) or stats.dtype != torch.float32 or stats.device != dev or not stats.is_contiguous():
+        raise ValueError(f"stats must be contiguous (2, {rows}) float32 on {dev}")
     gx = torch.empty(kept.shape, dtype=kept.dtype, device=dev)
     res, ldr = None, 0
     if g_residual is not None:
         res, _, _, ldr = _rows(_same(g_residual, gx, "g_residual"), "g_residual")
-    gw, gb = torch.empty(2, d, dtype=torch.float32, device=dev).unbind(0) if param_grads else (None, None)
-    with torch.cuda.device(dev):
-        n = nat.lib.bsrl_layernorm8_bwd_workspace_bytes(rows, d)
-        if n < 0:
-            raise nat.BsrlError(int(n), nat.last_error())
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        nat.check(nat.lib.bsrl_layernorm8_bwd(
-            m.data_ptr(), code, ld, _ptr(res), ldr, kept.codes.data_ptr(), kept.exps.data_ptr(), KINDS[kept.kind], mean.data_ptr(),
-            rstd.data_ptr(), weight.data_ptr(), rows, d, gx.data_ptr(), _DTYPES[kept.dtype], d, _ptr(gw), _ptr(gb), _ptr(ws), n, _stream(dev)))
+    gw = torch.empty(d, dtype=torch.float32, device=dev) if param_grads else None
+    gb = torch.empty(d, dtype=torch.float32, device=dev) if param_grads else None
+    n = _workspace_bytes("bsrl_layernorm8_bwd_workspace_bytes", dev.index, rows, d)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    at = stats.data_ptr()
+    _call(nat.lib.bsrl_layernorm8_bwd, dev, m.data_ptr(), code, ld, _ptr(res), ldr, kept._codes_ptr, kept._exps_ptr, KINDS[kept.kind], at,
+          at + 4 * rows, weight.data_ptr(), rows, d, gx.data_ptr(), _DTYPES[kept.dtype], d, _ptr(gw), _ptr(gb), _ptr(ws), n)
     return gx, gw, gb
 
 
@@ -255,7 +274,7 @@ class _LayerNorm8(Function):
     def forward(ctx, x, weight, bias, residual, eps, out_dtype, kind):
         ctx.set_materialize_grads(False)
         y, z, saved = layer_norm8_forward(x, weight, bias, eps, residual, out_dtype, kind)
-        ctx.save_for_backward(saved.kept.codes, saved.kept.exps, saved.mean, saved.rstd, weight)
+        ctx.save_for_backward(saved.kept.codes, saved.kept.exps, saved.stats, weight)
         ctx.kept = kind, saved.kept.shape, saved.kept.dtype
         ctx.y_dtype, ctx.has = y.dtype, (bias is not None, residual is not None)
         return (y, z) if residual is not None else y
@@ -263,12 +282,12 @@ class _LayerNorm8(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gy, gz=None):
-        codes, exps, mean, rstd, weight = ctx.saved_tensors
+        codes, exps, stats, weight = ctx.saved_tensors
         kept = Checkpoint8(codes, exps, *ctx.kept)
         if gy is None:
             gy = torch.zeros(kept.shape, dtype=ctx.y_dtype, device=kept.device)
         params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        gx, gw, gb = layer_norm8_backward(gy, LayerNorm8Saved(kept, mean, rstd), weight, gz, params)
+        gx, gw, gb = layer_norm8_backward(gy, LayerNorm8Saved(kept, stats), weight, gz, params)
         has_bias, has_residual = ctx.has
         return gx, gw, gb if has_bias else None, gx if has_residual else None, None, None, None
 
@@ -285,19 +304,16 @@ def linear8_weight_grad(gy: torch.Tensor, kept: Checkpoint8, bias: bool = True):
     """(g_weight (n, k), g_bias (n) or None) in fp32 of y = x w^T + b, from gy (..., n) float16 or bfloat16 and x (..., k) in 8 bits."""
     if gy.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"gy must be float16 or bfloat16, got {gy.dtype}")
-    if tuple(gy.shape[:-1]) != kept.shape[:-1] or gy.device != kept.device:
+    if gy.shape[:-1] != kept.shape[:-1] or gy.device != kept.device:
         raise ValueError(f"gy must be {kept.shape[:-1]} x n on {kept.device}, got {tuple(gy.shape)} on {gy.device}")
     m, rows, n, ld = _rows(gy, "gy")
     k, dev = kept.shape[-1], gy.device
     gw = torch.empty(n, k, dtype=torch.float32, device=dev)
     gb = torch.empty(n, dtype=torch.float32, device=dev) if bias else None
-    with torch.cuda.device(dev):
-        size = nat.lib.bsrl_linear8_wgrad_workspace_bytes(rows, n, k, int(m.data_ptr() % 16 == 0 and ld % 8 == 0))
-        if size < 0:
-            raise nat.BsrlError(int(size), nat.last_error())
-        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        nat.check(nat.lib.bsrl_linear8_wgrad(m.data_ptr(), _DTYPES[gy.dtype], ld, kept.codes.data_ptr(), kept.exps.data_ptr(), KINDS[kept.kind],
-                                             rows, n, k, gw.data_ptr(), _ptr(gb), _ptr(ws), size, _stream(dev)))
+    size = _workspace_bytes("bsrl_linear8_wgrad_workspace_bytes", dev.index, rows, n, k, int(m.data_ptr() % 16 == 0 and ld % 8 == 0))
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _call(nat.lib.bsrl_linear8_wgrad, dev, m.data_ptr(), _DTYPES[gy.dtype], ld, kept._codes_ptr, kept._exps_ptr, KINDS[kept.kind], rows, n, k,
+          gw.data_ptr(), _ptr(gb), _ptr(ws), size)
     return gw, gb
 
 
@@ -307,9 +323,8 @@ def _product(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor]) -> 
     n = w.shape[0]
     out = torch.empty(m, n, dtype=torch.float16, device=a.device)
     if m:
-        with torch.cuda.device(a.device):
-            nat.check(nat.lib.bsrl_linear(a.data_ptr(), w.data_ptr(), _ptr(bias), None, out.data_ptr(), 0, 0, m, n, k,
-                                          int(k % 64 == 0 and n % 16 == 0), _stream(a.device)))
+        _call(nat.lib.bsrl_linear, a.device, a.data_ptr(), w.data_ptr(), _ptr(bias), None, out.data_ptr(), 0, 0, m, n, k,
+              int(k % 64 == 0 and n % 16 == 0))
     return out
 
 

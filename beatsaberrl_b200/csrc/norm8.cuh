@@ -495,7 +495,8 @@ inline Shape shape_of(int d, bool aligned, bool bwd) {
   }
   return s;
 }
-inline int blocks_of(const Shape& s, int64_t rows) {
+inline int blocks_of(const Shape& s, int64_t rows, bool bwd) {
+  if (bwd && rows <= 4 * s.rows_per_block) return 1;         // its sums need no second kernel: a launch costs more than three turns
   const int64_t need = (rows + s.rows_per_block - 1) / s.rows_per_block, cap = (int64_t)sm_count() * s.resident;
   return (int)(need < cap ? need : cap);
 }
@@ -503,7 +504,7 @@ inline int blocks_of(const Shape& s, int64_t rows) {
 template <typename T, typename TY>
 int fwd(const FwdArgs<T, TY>& p, bool aligned, cudaStream_t stream);
 template <typename T, typename TY>
-int bwd(const BwdArgs<T, TY>& p, bool aligned, cudaStream_t stream);      // p.parts: blocks_of(shape_of(d, aligned, true), rows) rows of 2 d floats if that is above 1
+int bwd(const BwdArgs<T, TY>& p, bool aligned, cudaStream_t stream);      // p.parts: blocks_of(shape_of(d, aligned, true), rows, true) rows of 2 d floats if that is above 1
 
 // calls fn(TPR, NV, rows together if NV = 1 and a warp's lanes hold the row) for the shape
 template <typename Fn>
@@ -523,7 +524,7 @@ void with_shape(const Shape& s, Fn&& fn) {
 template <typename T, typename TY>
 int launch_fwd(const FwdArgs<T, TY>& p, bool aligned, cudaStream_t stream) {
   const Shape s = shape_of(p.d, aligned, false);
-  const int blocks = blocks_of(s, p.rows);
+  const int blocks = blocks_of(s, p.rows, false);
   with_shape(s, [&](auto TPR, auto NV) {
     constexpr int R = rows_together(NV());
     if (!aligned) launch_kernel(norm8_fwd_kernel<T, TY, false, true, TPR(), NV(), R>, blocks, s.threads, 0, stream, p);
@@ -536,7 +537,7 @@ int launch_fwd(const FwdArgs<T, TY>& p, bool aligned, cudaStream_t stream) {
 template <typename T, typename TY>
 int launch_bwd(const BwdArgs<T, TY>& p, bool aligned, cudaStream_t stream) {
   const Shape s = shape_of(p.d, aligned, true);
-  const int blocks = blocks_of(s, p.rows);
+  const int blocks = blocks_of(s, p.rows, true);
   const size_t smem = s.tpr > 0 ? 2 * p.d * sizeof(float) : 0;
   with_shape(s, [&](auto TPR, auto NV) {
     constexpr int R = rows_together(NV());

@@ -88,12 +88,12 @@ int norm8_fwd(const Norm8Args& a, cudaStream_t stream) {
 }
 
 int64_t norm8_bwd_workspace(int64_t rows, int d) {
-  const int blocks = blocks_of(shape_of(d, true, true), rows);            // the backward shares out both kinds of rows alike
+  const int blocks = blocks_of(shape_of(d, true, true), rows, true);            // the backward shares out both kinds of rows alike
   return blocks > 1 ? (int64_t)blocks * 2 * d * (int64_t)sizeof(float) : 0;
 }
 int norm8_bwd(const Norm8BwdArgs& a, float* workspace, cudaStream_t stream) {
   const bool aligned = bwd_by16(a);
-  const int blocks = blocks_of(shape_of(a.d, aligned, true), a.rows);
+  const int blocks = blocks_of(shape_of(a.d, aligned, true), a.rows, true);
   float* parts = blocks > 1 && (a.g_gamma || a.g_beta) ? workspace : nullptr;
   int rc;
   if (a.dtype == BSRL_F16) rc = run_bwd<__half, __half>(a, aligned, parts, stream);
