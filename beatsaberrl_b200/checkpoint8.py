@@ -224,7 +224,8 @@ def layer_norm8_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[to
     """LayerNorm over the last dimension of z = x + residual (rounded to x's type): (y, z, saved).
 
     weight and bias are fp32.  y has ``out_dtype`` (default: x's type): any of the three for fp32 rows, their own for 16-bit ones.
-    Without a residual z is x.  Rows are at most 8,192 wide."""
+    Without a residual z is x.  Rows are at most 8,192 wide.  What is kept is z: rows whose mean lies far beyond their spread keep little
+    of the spread."""
     code, k = _dtype(x, "x"), _kind(kind)
     m, rows, d, ld = _rows(x, "x")
     dev = x.device

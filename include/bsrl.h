@@ -319,6 +319,8 @@ int bsrl_gelu8_bwd(const void* gy, int32_t dtype, int64_t ldgy, const uint8_t* c
  * bsrl_layernorm8_bwd, with h = (z8 - mean) rstd and gh = gy gamma:
  *   gx = rstd (gh - mean(gh) - h mean(gh h)) (+ g_residual, the gradient that reaches z by other ways; may be NULL), in `dtype`
  *   g_gamma = sum over rows of gy h, g_beta = sum over rows of gy (written, not added to; either may be NULL)
+ * The statistics are those of z itself, h is as near to the normalised z as the checkpoint to z in units of the row's spread: a row
+ * that spreads by less than its blocks' step (a mean far beyond its variance; a single element) has little of a gradient left.
  * gx is the gradient of x and of the residual.  gx may be g_residual, or gy where the types agree.  workspace:
  * bsrl_layernorm8_bwd_workspace_bytes() of device memory, 16-byte aligned (0 bytes: may be NULL). */
 int bsrl_layernorm8(const void* x, const void* residual, int32_t dtype, int64_t ldx, int64_t ldr, const float* gamma,
