@@ -2,14 +2,15 @@
 //   g_weight (n, k) = g^T x8,  g_bias (n) = column sums of g,  over `rows` rows; g 16-bit, results fp32.
 //
 // Persistent, warp-specialised tcgen05 kernel, one CTA per SM or (CTAS = 2) pairs of CTAs on neighbouring SMs.  The contraction runs
-// over rows, so both operands are MN-major tiles of 64 rows as they lie in memory; a tile of the result has 128 CTAS x BN elements:
-//   warp 0        TMA producer of g: 64 rows x the CTA's own 128 columns per stage, columns and rows past the ends as zeros;
+// over rows, so both operands are MN-major tiles of 64 rows as they lie in memory; a tile of the result has 128 CTAS MH x BN elements:
+//   warp 0        TMA producer of g: 64 rows x the CTA's own 128 MH columns per stage, columns and rows past the ends as zeros;
 //   warp 1        MMA issuer (a pair's leader's), into one of two accumulators of BN columns in TMEM;
-//   warps 2..17   converters: 16 codes per 16-byte load to the 16-bit type of g (exact: the scale is a power of two), into the swizzled
-//                 tile that the MMAs (of both CTAs) read.  Groups of warps take stages in turn and request a stage's codes before they wait for its
-//                 slot, so several stages' loads are under way;
-//   warps 18..21  drain: accumulators to the workspace while the next chain runs into the other accumulator;
-//   warps 22..25  column sums of g from the stage, for the first column tile's work items only (no second read of g).
+//   converters    16 codes per 16-byte load to the 16-bit type of g (exact: the scale is a power of two), into the swizzled tile that the
+//                 MMAs (of both CTAs) read.  Groups of warps take stages in turn and request a stage's codes before they wait for its slot, so several
+//                 stages' loads are under way;
+//   drain         accumulators to the workspace while the next chain runs into the other set (one set where a CTA has two accumulators
+//                 beside each other: the MMAs wait);
+//   column sums   of g from the stage, for the first column tile's work items only (no second read of g).
 // Why groups: the proxy fence ahead of a converter's arrival waits for all loads its thread has in flight, so a thread cannot hold the
 // next stages' codes in registers (that took 2,150 cycles a stage, a load's latency each).  Codes through a TMA ring instead cost the shared
 // memory 16 KB a stage, which is what bounds the kernel together with the issue slots: 1,310 cycles a stage with column sums, 1,030 without.
@@ -33,23 +34,31 @@ using namespace p8;
 constexpr int KERNEL_ID = 14;
 constexpr int BK = 64;                           // rows per stage
 constexpr int BLOCK_BYTES = BK * 128;            // 64 columns x 64 rows of 16 bits
-constexpr int G_BYTES = 2 * BLOCK_BYTES;         // 128 columns of g
-constexpr int CONV_WARPS = 16, DRAIN_WARPS = 4, SUM_WARPS = 4;
-constexpr int groups_of(int ctas) { return ctas == 2 ? 4 : 2; }                // of converters, which take stages in turn
-constexpr int sum_groups(int ctas) { return ctas == 2 ? 4 : 2; }               // of sum warps, likewise
-constexpr int CONV0 = 2, DRAIN0 = CONV0 + CONV_WARPS, SUM0 = DRAIN0 + DRAIN_WARPS;      // first warp of each role
-constexpr int THREADS = (SUM0 + SUM_WARPS) * 32;
 constexpr int MAX_BN = 256;
 constexpr int TMEM_COLS = 2 * MAX_BN;
+#ifndef COST1
+#define COST1 3.1
+#define COST2 4.6
+#endif
 constexpr int kChain = 32;                       // stages between drains: 2,048 rows
-constexpr int PHASES = SUM_WARPS * 32 / 16;      // threads that share eight columns of g
-constexpr int stages_of(int ctas) { return ctas == 2 ? 6 : 4; }
-constexpr int stage_bytes(int ctas) { return G_BYTES + 4 / ctas * BLOCK_BYTES; }
-constexpr int smem_bytes(int ctas) { return stages_of(ctas) * stage_bytes(ctas) + 1024 /*alignment*/ + 512 /*barriers*/; }
-// A group that has seen stage i - groups knows that the slot of stage i has been through stage i - stages_of: without that its wait could
-// take the phase before the last one for the last one
-static_assert(groups_of(1) <= stages_of(1) && groups_of(2) <= stages_of(2) && sum_groups(1) <= stages_of(1) && sum_groups(2) <= stages_of(2), "phases");
-static_assert(smem_bytes(1) <= 227 * 1024 && smem_bytes(2) <= 227 * 1024, "shared memory");
+
+// CTAS: 1, or 2: a pair.  MH: accumulators of 128 columns of g beside each other per CTA.
+template <int CTAS, int MH>
+struct Form {
+  static constexpr int G_BYTES = 2 * MH * BLOCK_BYTES, STAGE_BYTES = G_BYTES + 4 / CTAS * BLOCK_BYTES;
+  static constexpr int STAGES = CTAS == 1 ? 4 : MH == 1 ? 6 : 4;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 /*alignment*/ + 512 /*barriers*/;
+  static constexpr int BUFS = 2 / MH;                                          // sets of accumulators in TMEM
+  // Converters take stages in turn, a group each; sum warps likewise.  A group always has the same slots of the ring: its waits, by parity, are
+  // for consecutive phases of their barriers.  (Groups that do not divide the stages meet a slot every other time, and slots are freed out of
+  // order where the sums lag: a wait could then take the phase before the last one for the last one.)
+  static constexpr int CONV_WARPS = CTAS == 1 ? 16 : MH == 1 ? 12 : 8, GROUPS = CTAS == 1 ? 2 : CONV_WARPS / 4;
+  static constexpr int SUM_WARPS = MH == 1 && CTAS == 2 ? 6 : 4, SUM_GROUPS = CTAS == 1 ? 2 : SUM_WARPS;
+  static_assert(STAGES % GROUPS == 0 && STAGES % SUM_GROUPS == 0, "phases");
+  static constexpr int CHUNKS = 16 * MH, PHASES = SUM_WARPS * 32 / CHUNKS;     // pieces of eight columns of g; threads that share one
+  static constexpr int CONV0 = 2, DRAIN0 = CONV0 + CONV_WARPS, SUM0 = DRAIN0 + 4 * MH, THREADS = (SUM0 + SUM_WARPS) * 32;      // first warp of each role
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
 
 struct Shared {
   uint64_t full_g[6], full_x[6], empty[6], acc_full[2], acc_empty[2], mma_done;
@@ -68,10 +77,10 @@ struct Args {
   int64_t rows;
   int64_t pitch;                 // of the codes
   int bn;                        // columns of a tile of x
-  int n_tiles, k_tiles, splits;
+  int n_tiles, k_tiles, splits;    // n tiles of 128 CTAS MH columns of g
   int k_blocks;                  // stages of all rows
-  float* parts;                  // (tiles, splits, 4 CTAS, bn / 4, 32 rows, 4 columns)
-  float* bias_parts;             // (splits, PHASES, n_tiles x 128 CTAS), nullptr: no column sums
+  float* parts;                  // (tiles, splits, 4 CTAS MH, bn / 4, 32 rows, 4 columns)
+  float* bias_parts;             // (splits, PHASES, n_tiles x 128 CTAS MH), nullptr: no column sums
 };
 
 // Item w -> (split, n tile, k tile), split-major: the tiles of the same rows run at the same time
@@ -151,12 +160,13 @@ __device__ __forceinline__ void convert16(const uint4& code, uint32_t e, uint32_
   }
 }
 
-template <typename TG, int KIND, int CTAS>
-__global__ void __launch_bounds__(THREADS, 1)
+template <typename TG, int KIND, int CTAS, int MH>
+__global__ void __launch_bounds__(Form<CTAS, MH>::THREADS, 1)
 wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
+  using F = Form<CTAS, MH>;
   constexpr bool PAIR = CTAS == 2;
-  constexpr int STAGES = stages_of(CTAS), STAGE_BYTES = stage_bytes(CTAS);
-  constexpr int GROUPS = groups_of(CTAS), GROUP_WARPS = CONV_WARPS / GROUPS;
+  constexpr int STAGES = F::STAGES, STAGE_BYTES = F::STAGE_BYTES, G_BYTES = F::G_BYTES;
+  constexpr int GROUPS = F::GROUPS, GROUP_WARPS = F::CONV_WARPS / GROUPS, CONV0 = F::CONV0, DRAIN0 = F::DRAIN0, SUM0 = F::SUM0;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -173,11 +183,11 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&sh->full_g[s]), 1);
       mbar_init(smem_u32(&sh->full_x[s]), CTAS * GROUP_WARPS);       // the leader's: both CTAs' converters
-      mbar_init(smem_u32(&sh->empty[s]), 1 + (p.bias_parts ? SUM_WARPS / sum_groups(CTAS) : 0));
+      mbar_init(smem_u32(&sh->empty[s]), 1 + (p.bias_parts ? F::SUM_WARPS / F::SUM_GROUPS : 0));
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&sh->acc_full[b]), 1);
-      mbar_init(smem_u32(&sh->acc_empty[b]), CTAS * DRAIN_WARPS);   // the leader's: both CTAs' drain warps
+      mbar_init(smem_u32(&sh->acc_empty[b]), CTAS * 4 * MH);   // the leader's: both CTAs' drain warps
     }
     mbar_init(smem_u32(&sh->mma_done), 1);
     sh->abort = 0;
@@ -212,13 +222,13 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
       bool ok = true;
       for (int w = w_first; w < n_items && ok; w += w_step) {
         const Item m = item_of(w, p);
-        const int x = (m.nt * CTAS + rank) * 128;
+        const int x = (m.nt * CTAS + rank) * (128 * MH);
         for (int kb = m.kb0; kb < m.kb1; ++kb, ++it) {
           if (!mbar_wait(smem_u32(&sh->empty[s]), phase ^ 1, abort)) { give_up(sh, status, 1); ok = false; break; }
           const uint32_t bar = smem_u32(&sh->full_g[s]), dst = base + s * STAGE_BYTES;
           mbar_expect_tx(bar, G_BYTES);
-          tma_load_2d(dst, &tm_g, x, kb * BK, bar);
-          tma_load_2d(dst + BLOCK_BYTES, &tm_g, x + 64, kb * BK, bar);
+#pragma unroll
+          for (int b = 0; b < 2 * MH; ++b) tma_load_2d(dst + b * BLOCK_BYTES, &tm_g, x + b * 64, kb * BK, bar);
           if (++s == STAGES) { s = 0; phase ^= 1; }
         }
       }
@@ -250,16 +260,23 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
             tc_fence_after();
             const uint64_t g_desc = g0 + slot * (STAGE_BYTES >> 4), x_desc = x0 + slot * (STAGE_BYTES >> 4);
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k) {
-              if (PAIR) mma_f16_ss_pair(d, g_desc + 128 * k, x_desc + 128 * k, idesc, (i || k) ? 1u : 0u);
-              else mma_f16_ss(d, g_desc + 128 * k, x_desc + 128 * k, idesc, (i || k) ? 1u : 0u);
-            }
+            for (int h = 0; h < MH; ++h)
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k) {
+                const uint64_t g_at = g_desc + h * (2 * BLOCK_BYTES >> 4) + 128 * k;
+                if (PAIR) mma_f16_ss_pair(d + h * MAX_BN, g_at, x_desc + 128 * k, idesc, (i || k) ? 1u : 0u);
+                else mma_f16_ss(d + h * MAX_BN, g_at, x_desc + 128 * k, idesc, (i || k) ? 1u : 0u);
+              }
             PAIR ? tc_commit_pair(smem_u32(&sh->empty[slot])) : tc_commit(smem_u32(&sh->empty[slot]));
             if (++slot == STAGES) { slot = 0; phase ^= 1; }
           }
           if (ok) PAIR ? tc_commit_pair(smem_u32(&sh->acc_full[buf])) : tc_commit(smem_u32(&sh->acc_full[buf]));
-          acc_phase ^= buf;
-          buf ^= 1;
+          if (F::BUFS == 2) {
+            acc_phase ^= buf;
+            buf ^= 1;
+          } else {
+            acc_phase ^= 1;
+          }
         }
       }
       // every MMA issued must have retired before TMEM is freed (bounded, ignoring abort)
@@ -342,15 +359,15 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
     }
   } else if (warp < SUM0) {
     // ---------------------------------------------------------------- drain
-    const int quad = warp & 3;                         // TMEM lane quadrant this warp may read
+    const int quad = warp & 3, half = (warp - DRAIN0) >> 2;      // TMEM lane quadrant this warp may read; which accumulator
     uint32_t chains = 0;
     bool ok = true;
     for (int w = w_first; w < n_items && ok; w += w_step) {
       const Item m = item_of(w, p);
-      float* part = p.parts + (((int64_t)(m.nt * p.k_tiles + m.kt) * p.splits + m.split) * (4 * CTAS) + rank * 4 + quad) * (p.bn * 32) + lane * 4;
+      float* part = p.parts + (((int64_t)(m.nt * p.k_tiles + m.kt) * p.splits + m.split) * (4 * CTAS * MH) + (rank * MH + half) * 4 + quad) * (p.bn * 32) + lane * 4;
       for (int kb = m.kb0; kb < m.kb1; kb += kChain, ++chains) {
-        const int buf = chains & 1;
-        if (!mbar_wait_warp(smem_u32(&sh->acc_full[buf]), (chains >> 1) & 1, abort)) {
+        const int buf = F::BUFS == 2 ? chains & 1 : 0;
+        if (!mbar_wait_warp(smem_u32(&sh->acc_full[buf]), (F::BUFS == 2 ? chains >> 1 : chains) & 1, abort)) {
           if (lane == 0) give_up(sh, status, 8);
           ok = false;
           break;
@@ -362,7 +379,7 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
         // longer than a chain).
         for (int c = 0; c < p.bn; c += 32) {
           uint32_t r[32];
-          tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + buf * MAX_BN + c, r);
+          tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + (buf + half) * MAX_BN + c, r);
           tmem_wait_ld();
           float* out = part + c * 32;
 #pragma unroll
@@ -381,9 +398,9 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
     }
   } else if (p.bias_parts) {
     // ---------------------------------------------------------------- column sums of g
-    constexpr int SG = sum_groups(CTAS), LANES = SUM_WARPS * 32 / SG;          // a group takes every SG-th stage
+    constexpr int SG = F::SUM_GROUPS, LANES = F::SUM_WARPS * 32 / SG, CHUNKS = F::CHUNKS;      // a group takes every SG-th stage
     const int t = threadIdx.x - SUM0 * 32, group = t / LANES;
-    const int chunk = t & 15, first = (t % LANES) >> 4;        // eight columns, every (LANES / 16)-th row: a partial sum of its own
+    const int chunk = t % CHUNKS, first = (t % LANES) / CHUNKS;        // eight columns, every (LANES / CHUNKS)-th row: a partial sum of its own
     uint32_t s = 0, phase = 0, turn = 0;
     bool ok = true;
     for (int w = w_first; w < n_items && ok; w += w_step) {
@@ -401,7 +418,7 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
           if (m.kt == 0) {
             const uint8_t* blk = tiles_ptr + s * STAGE_BYTES + (chunk >> 3) * BLOCK_BYTES;
 #pragma unroll 8
-            for (int r = first; r < BK; r += LANES / 16) {
+            for (int r = first; r < BK; r += LANES / CHUNKS) {
               const uint4 v = *reinterpret_cast<const uint4*>(blk + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
               add_pair<TG>(v.x, acc[0], acc[1]);
               add_pair<TG>(v.y, acc[2], acc[3]);
@@ -416,7 +433,7 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
         if (++s == STAGES) { s = 0; phase ^= 1; }
       }
       if (ok && m.kt == 0) {
-        float4* out = reinterpret_cast<float4*>(p.bias_parts + (((int64_t)m.split * PHASES + (t >> 4)) * p.n_tiles + m.nt) * (128 * CTAS) + rank * 128 + chunk * 8);
+        float4* out = reinterpret_cast<float4*>(p.bias_parts + (((int64_t)m.split * F::PHASES + t / CHUNKS) * p.n_tiles + m.nt) * (128 * CTAS * MH) + rank * (128 * MH) + chunk * 8);
         out[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
         out[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
       }
@@ -441,7 +458,7 @@ struct AddArgs {
   float* gw;
   float* gb;
   int64_t ldw;
-  int n, k, bn, n_tiles, k_tiles, splits, ctas;
+  int n, k, bn, n_tiles, k_tiles, splits, tile_n, phases;      // tile_n: columns of g of a tile; phases: partial column sums of a split
   int64_t patches;
 };
 __global__ void __launch_bounds__(256) wgrad8_add_kernel(AddArgs p) {
@@ -449,11 +466,11 @@ __global__ void __launch_bounds__(256) wgrad8_add_kernel(AddArgs p) {
   __shared__ float patch[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (blockIdx.x >= p.patches) {             // 32 columns of g: a warp takes every eighth partial sum, then the warps' sums in order
-    const int c = (int)(blockIdx.x - p.patches) * 32 + lane, width = p.n_tiles * 128 * p.ctas;
+    const int c = (int)(blockIdx.x - p.patches) * 32 + lane, width = p.n_tiles * p.tile_n;
     float sum = 0.f;
     if (c < p.n) {
 #pragma unroll 8
-      for (int s = warp; s < p.splits * PHASES; s += 8) sum += p.bias_parts[(int64_t)s * width + c];
+      for (int s = warp; s < p.splits * p.phases; s += 8) sum += p.bias_parts[(int64_t)s * width + c];
     }
     patch[warp][lane] = sum;
     __syncthreads();
@@ -464,7 +481,7 @@ __global__ void __launch_bounds__(256) wgrad8_add_kernel(AddArgs p) {
     }
     return;
   }
-  const int chunks = p.bn / 32, blocks = 4 * p.ctas;
+  const int chunks = p.bn / 32, blocks = p.tile_n / 32;
   int64_t i = blockIdx.x;
   const int chunk = (int)(i % chunks);
   i /= chunks;
@@ -490,7 +507,7 @@ __global__ void __launch_bounds__(256) wgrad8_add_kernel(AddArgs p) {
   const int col = kt * p.bn + chunk * 32 + lane;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int row = nt * 128 * p.ctas + blk * 32 + warp + 8 * j;
+    const int row = nt * p.tile_n + blk * 32 + warp + 8 * j;
     if (row < p.n && col < p.k) p.gw[(int64_t)row * p.ldw + col] = patch[lane][warp + 8 * j];
   }
 }
@@ -505,8 +522,9 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* __restr
 
 // How a call is cut up
 struct Plan {
-  int ctas, bn, n_tiles, k_tiles, splits, k_blocks;
+  int ctas, mh, bn, n_tiles, k_tiles, splits, k_blocks, phases;
   bool copy;
+  int tile_n() const { return 128 * ctas * mh; }
   int64_t copy_bytes, parts_bytes, bias_bytes;
 };
 Plan plan_of(int64_t rows, int n, int k, bool copy) {
@@ -515,38 +533,52 @@ Plan plan_of(int64_t rows, int n, int k, bool copy) {
   best.copy = copy;
   const int sms = sm_count();
   double cost = 1e30;
-  for (int ctas = 1; ctas <= 2; ++ctas)
+  for (int form = 0; form < 3; ++form)
     for (int most = 64; most <= MAX_BN; most *= 2) {
+      const int ctas = form == 0 ? 1 : 2, mh = form == 2 ? 2 : 1;
       const int k_tiles = (k + most - 1) / most, bn = (int)round_up((k + k_tiles - 1) / k_tiles, 32 * ctas);
-      const int n_tiles = (n + 128 * ctas - 1) / (128 * ctas), units = sms / ctas;
+      const int n_tiles = (n + 128 * ctas * mh - 1) / (128 * ctas * mh), units = sms / ctas;
       const int64_t tiles = (int64_t)n_tiles * k_tiles;
       if (tiles > 1 << 20) continue;
-      // cycles of a stage and of a drain that nothing hides (an item's last); bytes of partial tiles, all SMs
-      const double stage = fmax(ctas == 2 ? 3.1 * bn : 4.0 * bn, 400.0), drain = 2000 + 12.0 * bn;
+      // cycles of a stage and of a drain that nothing hides (an item's last one; with one set of accumulators every one); bytes of partial tiles, all SMs
+      const double stage = fmax((form == 0 ? 4.0 : form == 1 ? COST1 : COST2) * bn, form == 2 ? 700.0 : 450.0), drain = 2000 + 8.0 * mh * bn;
       // pieces of the rows: as fill one or more waves of SMs, or stages of some length each
       for (int i = 0; i < 10; ++i) {
         int64_t splits = i < 4 ? (i + 1) * (int64_t)units / tiles : best.k_blocks >> (i - 4);
         splits = splits < 1 ? 1 : splits > best.k_blocks ? best.k_blocks : splits;
         if (splits > 2 * sms) continue;
         const double waves = (double)((tiles * splits + units - 1) / units), per = (double)((best.k_blocks + splits - 1) / splits);
-        const double c = waves * per * stage + drain + (double)tiles * splits * 128 * ctas * bn * 4 / 5000.0;
+        const double c = waves * (per * stage + (mh == 2 ? drain * ceil(per / kChain) : 0.0)) + drain + (double)tiles * splits * 128 * ctas * mh * bn * 4 / 5000.0;
         if (c < cost) {
           cost = c;
-          best.ctas = ctas; best.bn = bn; best.n_tiles = n_tiles; best.k_tiles = k_tiles; best.splits = (int)splits;
+          best.ctas = ctas; best.mh = mh; best.bn = bn; best.n_tiles = n_tiles; best.k_tiles = k_tiles; best.splits = (int)splits;
         }
       }
     }
+  best.phases = best.ctas == 1 ? Form<1, 1>::PHASES : best.mh == 1 ? Form<2, 1>::PHASES : Form<2, 2>::PHASES;
   best.copy_bytes = copy ? round_up(rows * round_up(n, 8) * 2, 256) : 0;
-  best.parts_bytes = round_up((int64_t)best.n_tiles * best.k_tiles * best.splits * 128 * best.ctas * best.bn * 4, 256);
-  best.bias_bytes = round_up((int64_t)best.splits * PHASES * best.n_tiles * 128 * best.ctas * 4, 256);
+  best.parts_bytes = round_up((int64_t)best.n_tiles * best.k_tiles * best.splits * best.tile_n() * best.bn * 4, 256);
+  best.bias_bytes = round_up((int64_t)best.splits * best.phases * best.n_tiles * best.tile_n() * 4, 256);
   return best;
 }
 
+template <typename TG, int KIND, int CTAS, int MH>
+int launch(const CUtensorMap& tm, const Args& p, int* status, cudaStream_t stream) {
+  using F = Form<CTAS, MH>;
+  static DeviceOnce once;
+  const int rc = once.run("wgrad8_kernel set-up", [] {
+    return cudaFuncSetAttribute(wgrad8_kernel<TG, KIND, CTAS, MH>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
+  });
+  if (rc != BSRL_OK) return rc;
+  const int items = p.n_tiles * p.k_tiles * p.splits, units = sm_count() / CTAS, grid = (items < units ? items : units) * CTAS;
+  launch_kernel<CTAS>(wgrad8_kernel<TG, KIND, CTAS, MH>, grid, F::THREADS, F::SMEM, stream, tm, p, status);
+  BSRL_LAUNCH_OK("wgrad8_kernel");
+  return BSRL_OK;
+}
 template <typename TG, int KIND>
-void launch(const Plan& pl, const CUtensorMap& tm, const Args& p, int* status, cudaStream_t stream) {
-  const int items = p.n_tiles * p.k_tiles * p.splits, units = sm_count() / pl.ctas, grid = (items < units ? items : units) * pl.ctas;
-  if (pl.ctas == 2) launch_kernel<2>(wgrad8_kernel<TG, KIND, 2>, grid, THREADS, smem_bytes(2), stream, tm, p, status);
-  else launch_kernel(wgrad8_kernel<TG, KIND, 1>, grid, THREADS, smem_bytes(1), stream, tm, p, status);
+int launch(const Plan& pl, const CUtensorMap& tm, const Args& p, int* status, cudaStream_t stream) {
+  return pl.ctas == 1 ? launch<TG, KIND, 1, 1>(tm, p, status, stream)
+         : pl.mh == 1 ? launch<TG, KIND, 2, 1>(tm, p, status, stream) : launch<TG, KIND, 2, 2>(tm, p, status, stream);
 }
 bool needs_copy(const void* g, int64_t ldg) { return !aligned16(g) || ldg % 8 != 0; }
 }  // namespace
@@ -578,23 +610,14 @@ int wgrad8(const void* g, int g_dtype, int64_t ldg, const uint8_t* codes, const 
   CUtensorMap tm;
   if (!make_tmap_f16(&tm, g, rows, n, ldg, BK)) return BSRL_ERR_CUDA;
   const Args p{codes, exps, rows, pitch_of(k), pl.bn, pl.n_tiles, pl.k_tiles, pl.splits, pl.k_blocks, parts, bias_parts};
-  static DeviceOnce once;
-  const int rc = once.run("wgrad8_kernel set-up", [] {
-    cudaError_t e = cudaSuccess;
-    for (auto* k : {wgrad8_kernel<__half, kInt8, 1>, wgrad8_kernel<__half, kE4m3, 1>, wgrad8_kernel<__nv_bfloat16, kInt8, 1>, wgrad8_kernel<__nv_bfloat16, kE4m3, 1>})
-      if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(1));
-    for (auto* k : {wgrad8_kernel<__half, kInt8, 2>, wgrad8_kernel<__half, kE4m3, 2>, wgrad8_kernel<__nv_bfloat16, kInt8, 2>, wgrad8_kernel<__nv_bfloat16, kE4m3, 2>})
-      if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(2));
-    return e;
-  });
-  if (rc != BSRL_OK) return rc;
   int* status = device_status_ptr();
   if (!status) return BSRL_ERR_CUDA;
-  if (g_dtype == BSRL_F16) kind == kInt8 ? launch<__half, kInt8>(pl, tm, p, status, stream) : launch<__half, kE4m3>(pl, tm, p, status, stream);
-  else kind == kInt8 ? launch<__nv_bfloat16, kInt8>(pl, tm, p, status, stream) : launch<__nv_bfloat16, kE4m3>(pl, tm, p, status, stream);
-  BSRL_LAUNCH_OK("wgrad8_kernel");
-  AddArgs a{parts, bias_parts, gw, gb, ldw, n, k, pl.bn, pl.n_tiles, pl.k_tiles, pl.splits, pl.ctas, 0};
-  a.patches = (int64_t)pl.n_tiles * pl.k_tiles * 4 * pl.ctas * (pl.bn / 32);
+  const int rc = g_dtype == BSRL_F16 ? (kind == kInt8 ? launch<__half, kInt8>(pl, tm, p, status, stream) : launch<__half, kE4m3>(pl, tm, p, status, stream))
+                                     : (kind == kInt8 ? launch<__nv_bfloat16, kInt8>(pl, tm, p, status, stream)
+                                                      : launch<__nv_bfloat16, kE4m3>(pl, tm, p, status, stream));
+  if (rc != BSRL_OK) return rc;
+  AddArgs a{parts, bias_parts, gw, gb, ldw, n, k, pl.bn, pl.n_tiles, pl.k_tiles, pl.splits, pl.tile_n(), pl.phases, 0};
+  a.patches = (int64_t)pl.n_tiles * pl.k_tiles * (pl.tile_n() / 32) * (pl.bn / 32);
   PdlScope overlap;
   pdl_enable();
   launch_kernel(wgrad8_add_kernel, (unsigned)(a.patches + (gb ? (n + 31) / 32 : 0)), 256, 0, stream, a);
