@@ -80,7 +80,7 @@ def _ptr(t: Optional[torch.Tensor]):
 def _call(fn, dev, *args) -> None:
     """fn(*args, stream) on the device's current stream.  The device is switched only where it is not the current one: with the context
     manager and a Stream object around every call the small ones took half as long again."""
-    if torch.cuda.current_device() == dev.index:
+    if torch._C._cuda_getDevice() == dev.index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):

@@ -4,7 +4,7 @@
 // Persistent, warp-specialised tcgen05 kernel, one CTA per SM or (CTAS = 2) pairs of CTAs on neighbouring SMs.  The contraction runs
 // over rows, so both operands are MN-major tiles of 64 rows as they lie in memory; a tile of the result has 128 CTAS MH x BN elements:
 //   warp 0        TMA producer of g: 64 rows x the CTA's own 128 MH columns per stage, columns and rows past the ends as zeros;
-//   warp 1        MMA issuer (a pair's leader's), into one of two accumulators of BN columns in TMEM;
+//   warp 1        MMA issuer (a pair's leader's), into one of two sets of accumulators of BN columns in TMEM;
 //   converters    16 codes per 16-byte load to the 16-bit type of g (exact: the scale is a power of two), into the swizzled tile that the
 //                 MMAs (of both CTAs) read.  Groups of warps take stages in turn and request a stage's codes before they wait for its slot, so several
 //                 stages' loads are under way;
@@ -17,8 +17,9 @@
 // A work item is (tile, piece of the rows).  The pieces' partial tiles go to the workspace and a second kernel adds them in order: the
 // same bits every time.  Inside an item the accumulators are drained every kChain stages and added in fp32, rounded to nearest: the tensor
 // core's own running sum truncates, about 2e-8 of the sum per 16 rows (475,136 rows in chains of 6,420 were 7.6e-6 off, of 2,048 2e-6).
-// A pair halves what a CTA converts and what its MMAs read of shared memory: with one CTA and two accumulators of 256 columns beside each
-// other (no second set to drain from) the shared memory's 128 bytes per cycle bound the stage, and every drain stopped the MMAs.
+// A pair halves what a CTA converts and what its MMAs read of shared memory; two accumulators per CTA halve the conversions per MMA again.
+// 475,136 x 1,024 x 256 (floor 170 us by bytes, 149 by FLOPs): one CTA 607 us, pairs 288, pairs with two accumulators 263 (282 with all
+// CTAs' drains at once, 232 with no drains but the last: the additions into L2 are what is left); 100,003 x 2,048 x 2,048: 1,860 / 898 / 734.
 // All waits are bounded (tc5.cuh); a wait that runs out sets the device status word and every role falls through to the teardown.
 #include <cmath>
 
@@ -36,11 +37,10 @@ constexpr int BK = 64;                           // rows per stage
 constexpr int BLOCK_BYTES = BK * 128;            // 64 columns x 64 rows of 16 bits
 constexpr int MAX_BN = 256;
 constexpr int TMEM_COLS = 2 * MAX_BN;
-#ifndef COST1
-#define COST1 3.1
-#define COST2 4.6
-#endif
-constexpr int kChain = 32;                       // stages between drains: 2,048 rows
+constexpr int kChain = 40;                       // stages between drains: 2,560 rows
+// An item's first chain: of another length for neighbouring items, so that the CTAs do not all drain at once (they add into L2 at its rate
+// for atomics, 4.8 TB/s, and the MMAs of two accumulators wait)
+__device__ __forceinline__ int first_chain(int item) { return kChain - (item % 8) * (kChain / 8); }
 
 // CTAS: 1, or 2: a pair.  MH: accumulators of 128 columns of g beside each other per CTA.
 template <int CTAS, int MH>
@@ -249,11 +249,12 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
       const uint64_t g0 = smem_desc_mn_sw128(base, BLOCK_BYTES), x0 = smem_desc_mn_sw128(base + G_BYTES, BLOCK_BYTES);
       for (int w = w_first; w < n_items && ok; w += w_step) {
         const Item m = item_of(w, p);
-        for (int left = m.kb1 - m.kb0; left > 0 && ok; left -= kChain) {
+        int n = 0;
+        for (int left = m.kb1 - m.kb0; left > 0 && ok; left -= n) {
           if (!mbar_wait<PAIR>(smem_u32(&sh->acc_empty[buf]), acc_phase, abort)) { give_up(sh, status, 3); ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem_base + buf * MAX_BN;
-          const int n = min(left, kChain);
+          n = min(left, n == 0 ? first_chain(w) : kChain);
           for (int i = 0; i < n; ++i) {
             // the converters' arrivals stand for g too
             if (!mbar_wait<PAIR>(smem_u32(&sh->full_x[slot]), phase, abort)) { give_up(sh, status, 4); ok = false; break; }
@@ -365,7 +366,7 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
     for (int w = w_first; w < n_items && ok; w += w_step) {
       const Item m = item_of(w, p);
       float* part = p.parts + (((int64_t)(m.nt * p.k_tiles + m.kt) * p.splits + m.split) * (4 * CTAS * MH) + (rank * MH + half) * 4 + quad) * (p.bn * 32) + lane * 4;
-      for (int kb = m.kb0; kb < m.kb1; kb += kChain, ++chains) {
+      for (int kb = m.kb0; kb < m.kb1; kb += kb == m.kb0 ? first_chain(w) : kChain, ++chains) {
         const int buf = F::BUFS == 2 ? chains & 1 : 0;
         if (!mbar_wait_warp(smem_u32(&sh->acc_full[buf]), (F::BUFS == 2 ? chains >> 1 : chains) & 1, abort)) {
           if (lane == 0) give_up(sh, status, 8);
@@ -541,7 +542,7 @@ Plan plan_of(int64_t rows, int n, int k, bool copy) {
       const int64_t tiles = (int64_t)n_tiles * k_tiles;
       if (tiles > 1 << 20) continue;
       // cycles of a stage and of a drain that nothing hides (an item's last one; with one set of accumulators every one); bytes of partial tiles, all SMs
-      const double stage = fmax((form == 0 ? 4.0 : form == 1 ? COST1 : COST2) * bn, form == 2 ? 700.0 : 450.0), drain = 2000 + 8.0 * mh * bn;
+      const double stage = fmax((form == 0 ? 4.0 : form == 1 ? 3.1 : 4.6) * bn, form == 2 ? 700.0 : 450.0), drain = 2000 + 8.0 * mh * bn;
       // pieces of the rows: as fill one or more waves of SMs, or stages of some length each
       for (int i = 0; i < 10; ++i) {
         int64_t splits = i < 4 ? (i + 1) * (int64_t)units / tiles : best.k_blocks >> (i - 4);
