@@ -8,6 +8,7 @@ using namespace bsrl;
 namespace {
 constexpr int64_t kMaxD = ((int64_t)1 << 31) - 64;
 constexpr int kMaxSide = 1 << 20;
+constexpr int64_t kMaxWeight = (int64_t)1 << 31;       // elements: keeps the numbers of tiles and work items in 32 bits
 
 int refuse(int status, const char* what, const char* why) {
   set_error("%s: %s", what, why);
@@ -139,8 +140,8 @@ int bsrl_layernorm8_bwd(const void* gy, int32_t gy_dtype, int64_t ldgy, const vo
 }
 
 int64_t bsrl_linear8_wgrad_workspace_bytes(int64_t rows, int32_t n, int32_t k, int32_t aligned) {
-  if (rows < 0 || rows > 0x7fffff00 - 1 || n < 1 || k < 1 || n > kMaxSide || k > kMaxSide) {
-    set_error("linear8_wgrad: rows must be 0 .. 2^31 - 257, n and k 1 .. 2^20");
+  if (rows < 0 || rows > 0x7fffff00 - 1 || n < 1 || k < 1 || n > kMaxSide || k > kMaxSide || (int64_t)n * k > kMaxWeight) {
+    set_error("linear8_wgrad: rows must be 0 .. 2^31 - 257, n and k 1 .. 2^20, n k at most 2^31");
     return -1;
   }
   return rows == 0 ? 0 : wgrad8_workspace(rows, n, k, aligned != 0);
@@ -149,8 +150,8 @@ int64_t bsrl_linear8_wgrad_workspace_bytes(int64_t rows, int32_t n, int32_t k, i
 int bsrl_linear8_wgrad(const void* gy, int32_t gy_dtype, int64_t ldgy, const uint8_t* codes, const uint8_t* exps, int32_t kind, int64_t rows,
                        int32_t n, int32_t k, float* g_weight, float* g_bias, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* me = "linear8_wgrad";
-  if (rows < 0 || rows > 0x7fffff00 - 1 || n < 1 || k < 1 || n > kMaxSide || k > kMaxSide)
-    return refuse(BSRL_ERR_SHAPE, me, "rows must be 0 .. 2^31 - 257, n and k 1 .. 2^20");
+  if (rows < 0 || rows > 0x7fffff00 - 1 || n < 1 || k < 1 || n > kMaxSide || k > kMaxSide || (int64_t)n * k > kMaxWeight)
+    return refuse(BSRL_ERR_SHAPE, me, "rows must be 0 .. 2^31 - 257, n and k 1 .. 2^20, n k at most 2^31");
   CHECK(check_rows(me, gy, gy_dtype, ldgy, rows, n));
   CHECK(check_kept(me, codes, exps, kind, rows));
   if (gy_dtype == BSRL_F32) return refuse(BSRL_ERR_UNSUPPORTED, me, "gy must be f16 or bf16");

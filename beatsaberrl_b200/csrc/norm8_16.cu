@@ -42,28 +42,28 @@ __global__ void __launch_bounds__(1024) add_parts_kernel(const float* __restrict
 
 namespace {
 using namespace norm8;
-// whether every row of every operand can be taken 16 bytes at a time
+// whether every row of every operand starts on a whole piece: 16 bytes, fp32 32
 struct Rows {
   const void* base;
   int64_t ld;
   int size;
 };
-bool by16(int d, std::initializer_list<Rows> all) {
+bool on_pieces(int d, std::initializer_list<Rows> all) {
   if (d % 8) return false;
   for (const Rows& r : all)
-    if (r.base && (!aligned16(r.base) || (r.ld * r.size) % 16)) return false;
+    if (r.base && (reinterpret_cast<uintptr_t>(r.base) % (8 * r.size) || r.ld % 8)) return false;
   return true;
 }
 template <typename T, typename TY>
 int run_fwd(const Norm8Args& a, cudaStream_t stream) {
   const FwdArgs<T, TY> p{static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<T*>(a.z), static_cast<TY*>(a.y), a.gamma, a.beta,
                          a.codes, a.exps, a.mean, a.rstd, a.rows, a.ldx, a.ldr, a.ldz, a.ldy, a.d, a.kind, a.eps};
-  const bool aligned = by16(a.d, {{a.x, a.ldx, sizeof(T)}, {a.residual, a.ldr, sizeof(T)}, {a.z, a.ldz, sizeof(T)}, {a.y, a.ldy, sizeof(TY)}, {a.gamma, 4, 4}, {a.beta, 4, 4}});
+  const bool aligned = on_pieces(a.d, {{a.x, a.ldx, sizeof(T)}, {a.residual, a.ldr, sizeof(T)}, {a.z, a.ldz, sizeof(T)}, {a.y, a.ldy, sizeof(TY)}, {a.gamma, 8, 4}, {a.beta, 8, 4}});
   return fwd<T, TY>(p, aligned, stream);
 }
-bool bwd_by16(const Norm8BwdArgs& a) {
+bool bwd_on_pieces(const Norm8BwdArgs& a) {
   const int t = a.dtype == BSRL_F32 ? 4 : 2, ty = a.gy_dtype == BSRL_F32 ? 4 : 2;
-  return by16(a.d, {{a.gy, a.ldgy, ty}, {a.g_residual, a.ldgr, t}, {a.gx, a.ldgx, t}, {a.gamma, 4, 4}});
+  return on_pieces(a.d, {{a.gy, a.ldgy, ty}, {a.g_residual, a.ldgr, t}, {a.gx, a.ldgx, t}, {a.gamma, 8, 4}});
 }
 template <typename T, typename TY>
 int run_bwd(const Norm8BwdArgs& a, bool aligned, float* parts, cudaStream_t stream) {
@@ -92,7 +92,7 @@ int64_t norm8_bwd_workspace(int64_t rows, int d) {
   return blocks > 1 ? (int64_t)blocks * 2 * d * (int64_t)sizeof(float) : 0;
 }
 int norm8_bwd(const Norm8BwdArgs& a, float* workspace, cudaStream_t stream) {
-  const bool aligned = bwd_by16(a);
+  const bool aligned = bwd_on_pieces(a);
   const int blocks = blocks_of(shape_of(a.d, aligned, true), a.rows, true);
   float* parts = blocks > 1 && (a.g_gamma || a.g_beta) ? workspace : nullptr;
   int rc;

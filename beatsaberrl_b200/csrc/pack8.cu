@@ -80,11 +80,14 @@ __device__ __forceinline__ void gelu_slopes(const float (&x)[8], float (&s)[8]) 
   }
 }
 
+// How the rows lie: all as one dense row; rows that 16 bytes divide; any
+enum Rows { kFlat, kAligned, kAny };
 template <typename T>
-constexpr int unroll_of(bool aligned) { return sizeof(T) == 4 || !aligned ? 2 : 4; }
-template <int OP, typename T, int KIND, bool ALIGNED>
+constexpr int unroll_of(int mode) { return sizeof(T) == 4 || mode == kAny ? 2 : 4; }
+template <int OP, typename T, int KIND, int MODE>
 __global__ void __launch_bounds__(kThreads) elem8_kernel(ElemArgs p) {
-  constexpr int U = unroll_of<T>(ALIGNED);
+  constexpr int U = unroll_of<T>(MODE);
+  constexpr bool ALIGNED = MODE != kAny;
   constexpr bool READS_CODES = OP == kExpand || OP == kGeluBwd;
   const int64_t per_row = pitch_of(p.d) / 8;
   const Span span_in = OP != kExpand && !ALIGNED ? span_of(static_cast<const T*>(p.in), p.rows, p.d, p.ld_in) : Span{};
@@ -101,11 +104,12 @@ __global__ void __launch_bounds__(kThreads) elem8_kernel(ElemArgs p) {
       const int64_t i = first + u * kThreads;
       int64_t row = 0, col = i * 8;
       piece[u] = 1;
-      if (p.rows > 1) {
+      if (MODE != kFlat && p.rows > 1) {
         row = div_index(i, (int)per_row, &piece[u]);
         col = (int64_t)piece[u] * 8;
       }
-      live[u] = i >= p.pieces || col >= p.d ? 0 : p.d - col < 8 ? (int)(p.d - col) : 8;
+      if (MODE == kFlat) live[u] = i < p.pieces ? 8 : 0;
+      else live[u] = i >= p.pieces || col >= p.d ? 0 : p.d - col < 8 ? (int)(p.d - col) : 8;
       out_at[u] = row * p.ld_out + col;
       if (OP != kExpand) {
         const T* from = static_cast<const T*>(p.in) + row * p.ld_in + col;
@@ -174,16 +178,19 @@ __global__ void __launch_bounds__(kThreads) elem8_kernel(ElemArgs p) {
   }
 }
 
-template <int OP, typename T, int KIND, bool ALIGNED>
+template <int OP, typename T, int KIND, int MODE>
 void launch(const ElemArgs& p, cudaStream_t stream) {
-  constexpr int U = unroll_of<T>(ALIGNED);
+  constexpr int U = unroll_of<T>(MODE);
   const int64_t tiles = (p.pieces + kThreads * U - 1) / (kThreads * U), cap = (int64_t)sm_count() * 32;
-  launch_kernel(elem8_kernel<OP, T, KIND, ALIGNED>, (unsigned)(tiles < cap ? tiles : cap), kThreads, 0, stream, p);
+  launch_kernel(elem8_kernel<OP, T, KIND, MODE>, (unsigned)(tiles < cap ? tiles : cap), kThreads, 0, stream, p);
+}
+template <int OP, typename T, int KIND>
+void pick(const ElemArgs& p, int mode, cudaStream_t stream) {
+  mode == kFlat ? launch<OP, T, KIND, kFlat>(p, stream) : mode == kAligned ? launch<OP, T, KIND, kAligned>(p, stream) : launch<OP, T, KIND, kAny>(p, stream);
 }
 template <int OP, typename T>
-void pick(const ElemArgs& p, int kind, bool aligned, cudaStream_t stream) {
-  if (kind == kInt8) aligned ? launch<OP, T, kInt8, true>(p, stream) : launch<OP, T, kInt8, false>(p, stream);
-  else aligned ? launch<OP, T, kE4m3, true>(p, stream) : launch<OP, T, kE4m3, false>(p, stream);
+void pick(const ElemArgs& p, int kind, int mode, cudaStream_t stream) {
+  kind == kInt8 ? pick<OP, T, kInt8>(p, mode, stream) : pick<OP, T, kE4m3>(p, mode, stream);
 }
 template <int OP>
 int run(const void* in, int64_t ld_in, void* out, int64_t ld_out, int dtype, int64_t rows, int64_t d, int kind, uint8_t* codes,
@@ -194,12 +201,14 @@ int run(const void* in, int64_t ld_in, void* out, int64_t ld_out, int dtype, int
     rows = 1;
     ld_in = ld_out = d;
   }
-  auto by16 = [&](const void* base, int64_t ld) { return !base || (aligned16(base) && (rows == 1 || (ld * size) % 16 == 0)); };
-  const bool aligned = d % 8 == 0 && by16(in, ld_in) && by16(out, ld_out);
+  const int unit = 8 * size;                       // bytes of a piece: 16, fp32 32
+  auto on_units = [&](const void* base, int64_t ld) { return !base || (reinterpret_cast<uintptr_t>(base) % unit == 0 && (rows == 1 || (ld * size) % unit == 0)); };
+  const bool aligned = d % 8 == 0 && on_units(in, ld_in) && on_units(out, ld_out);
+  const int mode = !aligned ? kAny : rows == 1 && d % kBlock == 0 ? kFlat : kAligned;
   ElemArgs p{in, out, codes, exps, rows, d, ld_in, ld_out, rows * (pitch_of(d) / 8)};
-  if (dtype == BSRL_F32) pick<OP, float>(p, kind, aligned, stream);
-  else if (dtype == BSRL_F16) pick<OP, __half>(p, kind, aligned, stream);
-  else pick<OP, __nv_bfloat16>(p, kind, aligned, stream);
+  if (dtype == BSRL_F32) pick<OP, float>(p, kind, mode, stream);
+  else if (dtype == BSRL_F16) pick<OP, __half>(p, kind, mode, stream);
+  else pick<OP, __nv_bfloat16>(p, kind, mode, stream);
   BSRL_LAUNCH_OK(name);
   return BSRL_OK;
 }

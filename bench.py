@@ -596,6 +596,25 @@ def run_kernel(args):
         flops, nbytes = 2.0 * rows * n * k, rows * (n + k) * 2 + n * k * 4
         run = lambda: nat.check(nat.lib.bsrl_linear_bwd(gy.data_ptr(), x.data_ptr(), None, rows, n, k, gw.data_ptr(), None, None, 0,
                                                         scratch.data_ptr(), n_s, st))
+    elif args.kernel in ("layernorm8", "layernorm8_bwd", "gelu8", "gelu8_bwd", "wgrad8"):      # the forms that keep their input in 8 bits
+        from beatsaberrl_b200 import checkpoint8 as c8
+        kept_bytes = d + d / 32
+        if args.kernel.startswith("layernorm8"):
+            x, gy, lg, lb = rnd(rows, d), rnd(rows, d).half(), torch.ones(d).cuda(), torch.zeros(d).cuda()
+            _, _, saved = c8.layer_norm8_forward(x, lg, lb, out_dtype=torch.float16)
+            flops, nbytes = 20.0 * rows * d, rows * (6 * d + kept_bytes)
+            run = (lambda: c8.layer_norm8_backward(gy, saved, lg)) if args.kernel.endswith("bwd") else \
+                (lambda: c8.layer_norm8_forward(x, lg, lb, out_dtype=torch.float16))
+        elif args.kernel.startswith("gelu8"):
+            x = rnd(rows, d).half()
+            _, kept = c8.gelu8_forward(x)
+            flops, nbytes = 30.0 * rows * d, rows * (4 * d + kept_bytes)
+            run = (lambda: c8.gelu8_backward(x, kept)) if args.kernel.endswith("bwd") else (lambda: c8.gelu8_forward(x))
+        else:
+            n = args.cols or 4 * d
+            gy, kept = rnd(rows, n, scale=0.5).half(), c8.pack8(rnd(rows, d).half())
+            flops, nbytes = 2.0 * rows * n * d, rows * (2 * n + kept_bytes) + 4 * n * (d + 1)
+            run = lambda: c8.linear8_weight_grad(gy, kept)
     elif args.kernel == "update":     # one PPO update step (grad-mode forward + backward) on rows / 29 envs of the cfg2 model
         from beatsaberrl_b200.policy import NotePolicy
         from oracle import policy_oracle as po
@@ -685,7 +704,7 @@ def main():
     ap.add_argument("--no-recompute", action="store_true", help="skip the cfg5 PPO-recompute sub-record")
     ap.add_argument("--no-ref-gpu", action="store_true", help="skip the reference's GPU stream (1-GPU runs)")
     ap.add_argument("--kernel", default="", choices=("", "block_tail", "attn_block", "linear", "layernorm", "attention", "embed", "head_tail",
-                                                   "attention_tokens", "wgrad", "update", "linear_ln"),
+                                                   "attention_tokens", "wgrad", "update", "linear_ln", "layernorm8", "layernorm8_bwd", "gelu8", "gelu8_bwd", "wgrad8"),
                     help="time one kernel alone on --rows token rows instead of the whole forward")
     ap.add_argument("--rows", type=int, default=237568)
     ap.add_argument("--embed", type=int, default=256)

@@ -293,7 +293,7 @@ int bsrl_linear_bwd(const void* g_f16, const void* x_f16, const void* w_f16, int
  * Values have at most 8 significant bits: bf16 holds them exactly, fp16 as far as its range goes.
  *
  * Matrices have elements of BSRL_F32, BSRL_F16 or BSRL_BF16, rows `ld` elements apart (ld >= d) and no alignment but
- * their elements'; rows that start on 16 bytes, with d a multiple of 8, are faster.  rows may be 0.  d up to 2^31 - 64
+ * their elements'; rows that start on 16 bytes (f32: 32), with d a multiple of 8, are faster.  rows may be 0.  d up to 2^31 - 64
  * (bsrl_layernorm8: 8,192).  gamma, beta, mean, rstd and parameter gradients are fp32.  Sums are in fp32 and in one
  * order: a call on the same inputs gives the same bits.  Nothing may overlap except where said. */
 typedef enum bsrl_kind8 { BSRL_INT8 = 0, BSRL_E4M3 = 1 } bsrl_kind8;
@@ -334,7 +334,8 @@ int bsrl_layernorm8_bwd(const void* gy, int32_t gy_dtype, int64_t ldgy, const vo
 
 /* Weight and bias gradient of y = x w^T + b from x (rows, k) kept in 8 bits and gy (rows, n) f16 or bf16, on the tcgen05 tensor
  * cores: g_weight (n, k) = gy^T x8, g_bias (n) = column sums of gy (NULL: none); written, not added to.  x8 enters the product in
- * gy's type.  rows up to 2^31 - 257, n and k up to 2^20.  workspace: bsrl_linear8_wgrad_workspace_bytes() of device
+ * gy's type.  rows up to 2^31 - 257, n and k up to 2^20, n k up to
+ * 2^31.  Make the first call on a device outside any stream capture.  workspace: bsrl_linear8_wgrad_workspace_bytes() of device
  * memory, 256-byte aligned; `aligned` says that gy starts on 16 bytes and ldgy is a multiple of 8 (else the workspace also takes
  * a copy of gy that is). */
 int64_t bsrl_linear8_wgrad_workspace_bytes(int64_t rows, int32_t n, int32_t k, int32_t aligned);

@@ -83,7 +83,7 @@ WGRAD = dict(gy=A, gy_dtype=1, ldgy=64, codes=A, exps=A, kind=0, rows=100, n=64,
 
 @pytest.mark.parametrize("bad,status", [
     (dict(gy=None), NULL), (dict(g_weight=None), NULL), (dict(codes=None), NULL), (dict(rows=-1), SHAPE), (dict(rows=2 ** 31), SHAPE), (dict(n=0), SHAPE),
-    (dict(k=0), SHAPE), (dict(k=2 ** 20 + 1), SHAPE), (dict(ldgy=63), SHAPE), (dict(gy_dtype=0), UNSUPPORTED), (dict(gy=A + 1), ALIGN), (dict(g_weight=A + 2), ALIGN),
+    (dict(k=0), SHAPE), (dict(k=2 ** 20 + 1), SHAPE), (dict(n=2 ** 20, ldgy=2 ** 20, k=2049), SHAPE), (dict(ldgy=63), SHAPE), (dict(gy_dtype=0), UNSUPPORTED), (dict(gy=A + 1), ALIGN), (dict(g_weight=A + 2), ALIGN),
     (dict(workspace=None), WORKSPACE), (dict(workspace=A + 16), WORKSPACE), (dict(workspace_bytes=64), WORKSPACE)])
 def test_linear8_wgrad_refuses(native, bad, status):
     assert native.lib.bsrl_linear8_wgrad(*(WGRAD | bad).values(), None) == status
@@ -97,6 +97,7 @@ def test_workspace_sizes(native):
         a, b = size(rows, n, k, 1), size(rows, n, k, 0)
         assert 0 < a <= b and b - a >= rows * n * 2, (rows, n, k)
         assert a >= n * k * 4
+    assert size(2 ** 20, 2 ** 20, 2048, 1) > 0 and size(100, 2048, 2 ** 20, 1) > 0 and size(1, 2 ** 20, 2 ** 20, 1) == -1
     assert size(-1, 8, 8, 1) == -1 and size(2 ** 31, 8, 8, 1) == -1 and size(4, 0, 8, 1) == -1
     norm = native.lib.bsrl_layernorm8_bwd_workspace_bytes
     assert norm(1, 64) == 0 and norm(475136, 256) > 0 and norm(-1, 64) == -1 and norm(4, 8193) == -1
