@@ -178,7 +178,7 @@ __device__ __forceinline__ void load_any(Raw8<T>& r, const T* p, int n, const Sp
       const uint4 v = *reinterpret_cast<const uint4*>(from + j * 4);
       r.w[j] = v.x; r.w[j + 1] = v.y; r.w[j + 2] = v.z; r.w[j + 3] = v.w;
     }
-  } else if (n >= 8 && from >= s.lo && from + W * 4 + 16 <= s.hi) {
+  } else if (from >= s.lo && from + W * 4 + 16 <= s.hi) {
     uint32_t c[W + 4];
 #pragma unroll
     for (int j = 0; j < W + 4; j += 4) {
@@ -186,6 +186,13 @@ __device__ __forceinline__ void load_any(Raw8<T>& r, const T* p, int n, const Sp
       c[j] = v.x; c[j + 1] = v.y; c[j + 2] = v.z; c[j + 3] = v.w;
     }
     take_words<W, W == 4>(c, by, r.w);
+    if (n < 8) {                                   // what follows the row
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const int left = W == 8 ? 2 * (n - j) : n - 2 * j;       // halves of word j that belong to it
+        r.w[j] = left >= 2 ? r.w[j] : left == 1 ? r.w[j] & 0xffffu : 0u;
+      }
+    }
   } else {
     r.zero();
 #pragma unroll
