@@ -120,9 +120,10 @@ class Checkpoint8:
         for n in shape[:-1]:
             rows *= n
         blocks = -(-shape[-1] // BLOCK)
-        for t, cols, what in ((codes, blocks * BLOCK, "codes"), (exps, blocks, "exps")):
-            if t.dtype != torch.uint8 or t.shape != (rows, cols) or not t.is_contiguous():
-                raise ValueError(f"{what} must be contiguous ({rows}, {cols}) uint8, got {tuple(t.shape)} {t.dtype}")
+        if (codes.shape != (rows, blocks * BLOCK) or exps.shape != (rows, blocks) or codes.dtype != torch.uint8 or exps.dtype != torch.uint8
+                or not codes.is_contiguous() or not exps.is_contiguous()):
+            raise ValueError(f"codes and exps must be contiguous ({rows}, {blocks * BLOCK}) and ({rows}, {blocks}) uint8, got {tuple(codes.shape)} "
+                             f"{codes.dtype} and {tuple(exps.shape)} {exps.dtype}")
         if codes.device != exps.device:
             raise ValueError(f"codes and exps must be on one device, got {codes.device} and {exps.device}")
         if not codes.is_cuda:

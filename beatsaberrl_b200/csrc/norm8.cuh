@@ -462,7 +462,8 @@ __global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? kResident : 1) n
   }
 }
 
-constexpr int rows_together(int nv) { return nv == 1 ? 2 : 1; }
+// rows a team works on together (backward of 475,136 x 256: one 224 us, two 160, three 191, four 173; of 237,568 x 512: one 167, two 157)
+constexpr int rows_together(int tpr, int nv, bool bwd) { return nv == 1 || (bwd && tpr > 0) ? 2 : 1; }
 
 // How rows of d elements are shared out: lanes per team (TPR), steps per lane, rows worked on together
 struct Shape {
@@ -480,14 +481,14 @@ inline Shape shape_of(int d, bool aligned, bool bwd) {
   if (pieces <= (bwd || !aligned ? 64 : 128)) {
     s.tpr = pieces <= 4 ? 4 : pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
     s.nv = pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4;
-    s.r = rows_together(s.nv);
+    s.r = rows_together(s.tpr, s.nv, bwd);
     s.threads = kThreads;
     s.rows_per_block = kThreads / s.tpr * s.r;
     s.resident = kResident;
   } else {
     s.tpr = 0;
     s.nv = pieces <= 512 ? 1 : 2;
-    s.r = rows_together(s.nv);
+    s.r = rows_together(s.tpr, s.nv, bwd);
     s.threads = (int)round_up((pieces + s.nv - 1) / s.nv, 32);
     s.rows_per_block = s.r;
     s.resident = (bwd ? 512 : 1024) / s.threads;
@@ -526,7 +527,7 @@ int launch_fwd(const FwdArgs<T, TY>& p, bool aligned, cudaStream_t stream) {
   const Shape s = shape_of(p.d, aligned, false);
   const int blocks = blocks_of(s, p.rows, false);
   with_shape(s, [&](auto TPR, auto NV) {
-    constexpr int R = rows_together(NV());
+    constexpr int R = rows_together(TPR(), NV(), false);
     if (!aligned) launch_kernel(norm8_fwd_kernel<T, TY, false, true, TPR(), NV(), R>, blocks, s.threads, 0, stream, p);
     else if (p.res) launch_kernel(norm8_fwd_kernel<T, TY, true, true, TPR(), NV(), R>, blocks, s.threads, 0, stream, p);
     else launch_kernel(norm8_fwd_kernel<T, TY, true, false, TPR(), NV(), R>, blocks, s.threads, 0, stream, p);
@@ -540,11 +541,11 @@ int launch_bwd(const BwdArgs<T, TY>& p, bool aligned, cudaStream_t stream) {
   const int blocks = blocks_of(s, p.rows, true);
   const size_t smem = s.tpr > 0 ? 2 * p.d * sizeof(float) : 0;
   with_shape(s, [&](auto TPR, auto NV) {
-    constexpr int R = rows_together(NV());
+    constexpr int R = rows_together(TPR(), NV(), true);
     if constexpr (NV() <= 2) {
-    if (!aligned) launch_kernel(norm8_bwd_kernel<T, TY, false, true, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
-    else if (p.gres) launch_kernel(norm8_bwd_kernel<T, TY, true, true, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
-    else launch_kernel(norm8_bwd_kernel<T, TY, true, false, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
+      if (!aligned) launch_kernel(norm8_bwd_kernel<T, TY, false, true, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
+      else if (p.gres) launch_kernel(norm8_bwd_kernel<T, TY, true, true, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
+      else launch_kernel(norm8_bwd_kernel<T, TY, true, false, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
     }
   });
   BSRL_LAUNCH_OK("norm8_bwd_kernel");
