@@ -10,7 +10,7 @@ neighbouring values of a row share a power of two; ``kind`` "int8" is off by at 
 * ``pack8`` / ``Checkpoint8.expand``: any activation.
 
 Everything runs on the current stream of the tensors' device; nothing synchronises, and all memory comes from torch's allocator, so
-calls can be captured.  Gradients of parameters are fp32 sums in one order: the same inputs give the same bits.
+calls can be captured (make a first call on the device outside the capture).  Gradients of parameters are fp32 sums in one order: the same inputs give the same bits.
 """
 from __future__ import annotations
 
@@ -324,8 +324,15 @@ def linear8_weight_grad(gy: torch.Tensor, kept: Checkpoint8, bias: bool = True):
     return gw, gb
 
 
+def _on_16(t: torch.Tensor) -> torch.Tensor:
+    """t without gaps and from a 16-byte boundary on, as the products read it: a copy where it is not (a slice of something larger)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _product(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
     """a (m, k) w (n, k)^T + bias in fp16."""
+    a, w, bias = _on_16(a), _on_16(w), None if bias is None else _on_16(bias)
     m, k = a.shape
     n = w.shape[0]
     out = torch.empty(m, n, dtype=torch.float16, device=a.device)
@@ -339,9 +346,8 @@ class _Linear8(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, kind):
         n, k = weight.shape
-        a = x.reshape(-1, k).contiguous()
-        w = weight.to(torch.float16).contiguous()
-        y = _product(a, w, bias)
+        w = weight.to(torch.float16)
+        y = _product(x.reshape(-1, k), w, bias)
         kept = pack8(x, kind)
         ctx.save_for_backward(kept.codes, kept.exps, w)
         ctx.kept, ctx.w_dtype = (kind, kept.shape, kept.dtype), weight.dtype
@@ -356,7 +362,7 @@ class _Linear8(Function):
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         gx = gw = gb = None
         if need_x:
-            gx = _product(gy.reshape(-1, n).contiguous(), w.t().contiguous(), None).view(kept.shape)
+            gx = _product(gy.reshape(-1, n), w.t(), None).view(kept.shape)
         if need_w or need_b:
             gw, gb = linear8_weight_grad(gy, kept, need_b)
         return gx, gw.to(ctx.w_dtype) if need_w else None, gb, None
@@ -366,13 +372,13 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] 
     """Differentiable y = x weight^T + bias that keeps x in 8 bits.
 
     x (..., k) and y are float16, weight (n, k) float16 or a float32 master (rounded to float16 for the products; its gradient is
-    float32), bias (n) float32.  n and k multiples of 32 (the products' own limits)."""
+    float32), bias (n) float32.  n and k multiples of 32 (the products' own limits) up to 2^20."""
     if not x.is_cuda:
         raise RuntimeError("x must live on a CUDA device (this library has no CPU path)")
     if x.dtype != torch.float16 or weight.dtype not in (torch.float16, torch.float32):
         raise TypeError(f"x must be float16 and weight float16 or float32, got {x.dtype} and {weight.dtype}")
     if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1] or weight.device != x.device:
         raise ValueError(f"weight must be (n, {tuple(x.shape)[-1:]}) on {x.device}, got {tuple(weight.shape)} on {weight.device}")
-    if weight.shape[0] % 32 or weight.shape[1] % 32 or not weight.numel():
-        raise ValueError(f"weight's sides must be multiples of 32, got {tuple(weight.shape)}")
+    if weight.shape[0] % 32 or weight.shape[1] % 32 or not weight.numel() or max(weight.shape) > 1 << 20 or weight.numel() > 1 << 31:
+        raise ValueError(f"weight's sides must be multiples of 32 up to 2^20, their product at most 2^31, got {tuple(weight.shape)}")
     return _Linear8.apply(x, weight, _vector(bias, weight.shape[0], x.device, "bias"), kind)

@@ -393,7 +393,8 @@ def test_weight_gradient(c8, rows, n, k, dtype, kind):
     gw, gb = c8.linear8_weight_grad(gy, kept)
     xv = ref8(x, kind)[0].to(dtype).double()           # in fp16 the smallest values are rounded on their way into the product
     want, most = gy.double().t() @ xv, gy.double().abs().t() @ xv.abs()
-    # chains of 2,048 rows: a truncation (2 U) per 16 rows; their sums and the splits', rounded to nearest
+    # chains of at most 2,560 rows: a truncation (2 U) per 16 rows, 320 U; their sums and the splits', rounded to nearest: one per 2,560 rows, or
+    # up to 300 of shorter chains.  256 and 300 here cover both
     assert ((gw.double() - want).abs() <= most * (min(rows, 2048) / 16 * 2 + rows / 2048 + 300) * U + 1e-30).all()
     # a lane's share of the rows, then at most 8 x 300 partial sums by eights
     assert ((gb.double() - gy.double().sum(0)).abs() <= gy.double().abs().sum(0) * (rows / 8 + 400) * U + 1e-30).all()
@@ -605,3 +606,38 @@ def test_offsets_past_32_bits(c8):
     assert (gb == 3).all()
     want = alone.kept.expand().double().sum(0).expand(8, -1)
     assert ((gw.double() - want).abs() <= 20 * U * alone.kept.expand().double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype,out", [(F32, F16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("rows,d", [(1, 264), (3, 511), (33, 288), (1201, 512), (4801, 264), (2403, 509)])
+def test_layer_norm_of_rows_taken_by_twos(c8, rows, d, dtype, out, kind):
+    """Widths of 257 to 512: odd numbers of rows, one step and several per warp."""
+    g = gen(rows + 5 * d)
+    for name, x in layouts(rows, d, dtype, g, 2.0):
+        check_norm(c8, x, out, None, kind, g, name=name)
+        check_norm(c8, x, out, randn(rows, d, g=g, dtype=dtype), kind, g, name=name + "+residual")
+
+
+def test_linear_of_slices(c8):
+    """Inputs, weights, biases and gradients that start between 16-byte boundaries: the same results as of copies."""
+    g = gen(23)
+    for n, k in ((96, 64), (64, 96)):
+        flat = {"x": randn(40 * k + 3, g=g, dtype=F16), "w": randn(n * k + 5, g=g, dtype=F16), "b": randn(n + 1, g=g), "gy": randn(40 * n + 1, g=g, dtype=F16)}
+        odd = [flat["x"][3:].view(40, k), flat["w"][5:].view(n, k), flat["b"][1:], flat["gy"][1:].view(40, n)]
+        assert all(t.data_ptr() % 16 for t in odd)
+        results = []
+        for x, w, b, gy in (odd, [t.clone() for t in odd]):
+            x, w, b = (t.detach().requires_grad_() for t in (x, w, b))
+            with torch.enable_grad():
+                y = c8.linear8(x, w, b)
+                y.backward(gy)
+            results.append((y.detach(), x.grad, w.grad, b.grad))
+        for p, q in zip(*results):
+            assert torch.equal(p, q)
+        x, w, b, gy = (t.double() for t in odd)
+        # y: fp32 sums of k products (truncated: 2 U per 16 and rounding; k U covers the order), then half a step of fp16
+        most = x.abs() @ w.abs().t() + b.abs()
+        assert ((results[0][0].double() - (x @ w.t() + b)).abs() <= half_step(x @ w.t() + b, F16) + most * (k + 2) * U).all()
+        want = gy @ w
+        assert ((results[0][1].double() - want).abs() <= half_step(want, F16) + (gy.abs() @ w.abs()) * (n + 2) * U).all()
