@@ -9,7 +9,7 @@
 // of a warp up to 512 columns, a whole block above -- which holds it in registers between its one read and its one write, eight
 // neighbouring elements per lane and step.  Rows that 16 bytes do not divide are read by the aligned 16 bytes around a lane's piece and shifted
 // into place, and written the same way with the end of the neighbouring lane's piece.
-// 475,136 fp32 rows of 256 with fp16 results: 140 us forward (94 % of the copy rate), 163 backward (81 %).  What bounds the backward is the
+// 475,136 fp32 rows of 256 with fp16 results: 140 us forward (94 % of the copy rate), 160 backward (83 %).  What bounds the backward is the
 // instructions (220 per row and warp) and the 16 warps that its registers leave.  With twice the instructions (arithmetic one element at a
 // time, IEEE divisions) both took over 200 us whatever was requested ahead, in registers or through a ring in shared memory.
 //
@@ -135,9 +135,14 @@ __device__ __forceinline__ void store_piece(const Raw8<T>& r, T* row, int piece,
 }
 
 constexpr int kThreads = 256;                      // of blocks whose warps hold teams
-constexpr int block_threads(int tpr) { return tpr > 0 ? kThreads : 512; }
 // blocks of kThreads per SM: 128 registers each.  Three forward (80 registers, spills) 213 us where two are 176, of 475,136 rows of 256
 constexpr int kResident = 2;
+// Threads of blocks that hold a row, per SM, and blocks of kThreads: what registers are kept free for.  Unaligned rows run more warps than
+// aligned ones and one row at a time: they wait for what follows from what a piece's place in memory is.  60,007 x 1,001 fp16 with a residual, 512 / 768
+// threads: forward 240 / 201 us, backward 214 / 179; 100,003 x 509, two / three blocks: forward 197 / 170.  Aligned forward, 14,848 x 8,192 fp32, 512 / 1,024
+// threads 191 / 162 us; its backward 231 / 245.
+constexpr int block_threads(int tpr, bool aligned, bool bwd) { return tpr > 0 ? kThreads : !aligned ? 768 : bwd ? 512 : 1024; }
+constexpr int blocks_per_sm(int tpr, bool aligned, bool bwd) { return tpr == 0 ? 1 : aligned || bwd ? kResident : 3; }
 
 // This thread's part of the rows.  TPR > 0: TPR lanes of a warp hold a row; TPR = 0: the block does.  A warp or block takes ROWS rows at a time.
 template <int TPR, int R>
@@ -157,7 +162,7 @@ struct Place {
 
 // R: rows a team works on together.  NV: steps of eight elements that a lane takes of a row.  RES: there is a residual.
 template <typename T, typename TY, bool ALIGNED, bool RES, int TPR, int NV, int R>
-__global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? kResident : 1) norm8_fwd_kernel(FwdArgs<T, TY> p) {
+__global__ void __launch_bounds__(block_threads(TPR, ALIGNED, false), blocks_per_sm(TPR, ALIGNED, false)) norm8_fwd_kernel(FwdArgs<T, TY> p) {
   __shared__ float slots[2][32][4];
   int turn = 0;
   const Place<TPR, R> pl;
@@ -300,7 +305,7 @@ __global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? kResident : 1) n
 }
 
 template <typename T, typename TY, bool ALIGNED, bool RES, int TPR, int NV, int R>
-__global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? kResident : 1) norm8_bwd_kernel(BwdArgs<T, TY> p) {
+__global__ void __launch_bounds__(block_threads(TPR, ALIGNED, true), blocks_per_sm(TPR, ALIGNED, true)) norm8_bwd_kernel(BwdArgs<T, TY> p) {
   __shared__ float slots[2][32][4];
   extern __shared__ float s_sums[];                  // [2][d], teams of lanes only
   int turn = 0;
@@ -483,8 +488,9 @@ __global__ void __launch_bounds__(block_threads(TPR), TPR > 0 ? kResident : 1) n
   }
 }
 
-// rows a team works on together (backward of 475,136 x 256: one 224 us, two 160, three 191, four 173; of 237,568 x 512: one 167, two 157)
-constexpr int rows_together(int tpr, int nv, bool bwd) { return nv == 1 || (bwd && tpr > 0) ? 2 : 1; }
+// rows a team works on together (backward of 475,136 x 256: one 224 us, two 160, three 191, four 173; of 237,568 x 512: one 167, two 157; unaligned, of
+// 100,003 x 509: one 174, two 229)
+constexpr int rows_together(int tpr, int nv, bool aligned, bool bwd) { return aligned && (bwd ? nv == 1 || tpr > 0 : nv == 1 && tpr > 0) ? 2 : 1; }
 
 // How rows of d elements are shared out: lanes per team (TPR), steps per lane, rows worked on together
 struct Shape {
@@ -494,26 +500,24 @@ struct Shape {
   int resident;            // blocks per SM
 };
 constexpr int kMaxWidth = 8192;
-// Rows of 513 to 1,024: the forward of aligned ones by a warp's lanes (65,536 x 1,024 bf16 with a residual 109 us, a block 129), the backward by
-// blocks (118 us; a warp's lanes, with 64 running sums each, 202)
+// Rows above 512: by blocks (65,536 x 1,024 bf16 with a residual: forward 104 us, a warp's lanes with four pieces each 110; backward 113 / 202)
 inline Shape shape_of(int d, bool aligned, bool bwd) {
   const int pieces = (int)pitch_of(d) / 8;
   Shape s;
-  if (pieces <= (bwd || !aligned ? 64 : 128)) {
+  if (pieces <= 64) {
     s.tpr = pieces <= 4 ? 4 : pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
-    s.nv = pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4;
-    s.r = rows_together(s.tpr, s.nv, bwd);
+    s.nv = pieces <= 32 ? 1 : 2;
+    s.r = rows_together(s.tpr, s.nv, aligned, bwd);
     s.threads = kThreads;
     s.rows_per_block = kThreads / s.tpr * s.r;
-    s.resident = kResident;
+    s.resident = blocks_per_sm(s.tpr, aligned, bwd);
   } else {
     s.tpr = 0;
     s.nv = pieces <= 512 ? 1 : 2;
-    s.r = rows_together(s.tpr, s.nv, bwd);
+    s.r = rows_together(s.tpr, s.nv, aligned, bwd);
     s.threads = (int)round_up((pieces + s.nv - 1) / s.nv, 32);
     s.rows_per_block = s.r;
-    s.resident = (bwd ? 512 : 1024) / s.threads;
-    if (s.resident < 1) s.resident = 1;
+    s.resident = block_threads(0, aligned, bwd) / s.threads;
   }
   return s;
 }
@@ -528,7 +532,7 @@ int fwd(const FwdArgs<T, TY>& p, bool aligned, cudaStream_t stream);
 template <typename T, typename TY>
 int bwd(const BwdArgs<T, TY>& p, bool aligned, cudaStream_t stream);      // p.parts: blocks_of(shape_of(d, aligned, true), rows, true) rows of 2 d floats if that is above 1
 
-// calls fn(TPR, NV, rows together if NV = 1 and a warp's lanes hold the row) for the shape
+// calls fn(TPR, NV) for the shape
 template <typename Fn>
 void with_shape(const Shape& s, Fn&& fn) {
 #define BSRL_SHAPE(TPR_, NV_) \
@@ -538,7 +542,6 @@ void with_shape(const Shape& s, Fn&& fn) {
   BSRL_SHAPE(16, 1);
   BSRL_SHAPE(32, 1);
   BSRL_SHAPE(32, 2);
-  BSRL_SHAPE(32, 4);                                 // forward only
   BSRL_SHAPE(0, 1);
   BSRL_SHAPE(0, 2);
 #undef BSRL_SHAPE
@@ -548,8 +551,8 @@ int launch_fwd(const FwdArgs<T, TY>& p, bool aligned, cudaStream_t stream) {
   const Shape s = shape_of(p.d, aligned, false);
   const int blocks = blocks_of(s, p.rows, false);
   with_shape(s, [&](auto TPR, auto NV) {
-    constexpr int R = rows_together(TPR(), NV(), false);
-    if (!aligned) launch_kernel(norm8_fwd_kernel<T, TY, false, true, TPR(), NV(), R>, blocks, s.threads, 0, stream, p);
+    constexpr int R = rows_together(TPR(), NV(), true, false), R1 = rows_together(TPR(), NV(), false, false);
+    if (!aligned) launch_kernel(norm8_fwd_kernel<T, TY, false, true, TPR(), NV(), R1>, blocks, s.threads, 0, stream, p);
     else if (p.res) launch_kernel(norm8_fwd_kernel<T, TY, true, true, TPR(), NV(), R>, blocks, s.threads, 0, stream, p);
     else launch_kernel(norm8_fwd_kernel<T, TY, true, false, TPR(), NV(), R>, blocks, s.threads, 0, stream, p);
   });
@@ -562,12 +565,10 @@ int launch_bwd(const BwdArgs<T, TY>& p, bool aligned, cudaStream_t stream) {
   const int blocks = blocks_of(s, p.rows, true);
   const size_t smem = s.tpr > 0 ? 2 * p.d * sizeof(float) : 0;
   with_shape(s, [&](auto TPR, auto NV) {
-    constexpr int R = rows_together(TPR(), NV(), true);
-    if constexpr (NV() <= 2) {
-      if (!aligned) launch_kernel(norm8_bwd_kernel<T, TY, false, true, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
-      else if (p.gres) launch_kernel(norm8_bwd_kernel<T, TY, true, true, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
-      else launch_kernel(norm8_bwd_kernel<T, TY, true, false, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
-    }
+    constexpr int R = rows_together(TPR(), NV(), true, true), R1 = rows_together(TPR(), NV(), false, true);
+    if (!aligned) launch_kernel(norm8_bwd_kernel<T, TY, false, true, TPR(), NV(), R1>, blocks, s.threads, smem, stream, p);
+    else if (p.gres) launch_kernel(norm8_bwd_kernel<T, TY, true, true, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
+    else launch_kernel(norm8_bwd_kernel<T, TY, true, false, TPR(), NV(), R>, blocks, s.threads, smem, stream, p);
   });
   BSRL_LAUNCH_OK("norm8_bwd_kernel");
   return BSRL_OK;

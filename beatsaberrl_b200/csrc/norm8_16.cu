@@ -1,4 +1,6 @@
 // LayerNorm with its input kept in 8 bits: 16-bit rows (norm8.cuh), and the sum of the blocks' partial parameter gradients.
+#include <algorithm>
+
 #include "norm8.cuh"
 
 namespace bsrl {
@@ -88,7 +90,8 @@ int norm8_fwd(const Norm8Args& a, cudaStream_t stream) {
 }
 
 int64_t norm8_bwd_workspace(int64_t rows, int d) {
-  const int blocks = blocks_of(shape_of(d, true, true), rows, true);            // the backward shares out both kinds of rows alike
+  int blocks = 0;                                  // the more of aligned and unaligned rows
+  for (const bool aligned : {true, false}) blocks = std::max(blocks, blocks_of(shape_of(d, aligned, true), rows, true));
   return blocks > 1 ? (int64_t)blocks * 2 * d * (int64_t)sizeof(float) : 0;
 }
 int norm8_bwd(const Norm8BwdArgs& a, float* workspace, cudaStream_t stream) {
