@@ -18,7 +18,7 @@
 // same bits every time.  Inside an item the accumulators are drained every kChain stages and added in fp32, rounded to nearest: the tensor
 // core's own running sum truncates, about 2e-8 of the sum per 16 rows (475,136 rows in chains of 6,420 were 7.6e-6 off, of 2,048 2e-6).
 // A pair halves what a CTA converts and what its MMAs read of shared memory; two accumulators per CTA halve the conversions per MMA again.
-// 475,136 x 1,024 x 256 (floor 170 us by bytes, 149 by FLOPs): one CTA 607 us, pairs 288, pairs with two accumulators 263 (282 with all
+// 475,136 x 1,024 x 256 with chains of 2,560 rows (floor 170 us by bytes, 149 by FLOPs): one CTA 607 us, pairs 288, pairs with two accumulators 263 (282 with all
 // CTAs' drains at once, 232 with no drains but the last: the additions into L2 are what is left); 100,003 x 2,048 x 2,048: 1,860 / 898 / 734.
 // All waits are bounded (tc5.cuh); a wait that runs out sets the device status word and every role falls through to the teardown.
 #include <cmath>
@@ -37,10 +37,16 @@ constexpr int BK = 64;                           // rows per stage
 constexpr int BLOCK_BYTES = BK * 128;            // 64 columns x 64 rows of 16 bits
 constexpr int MAX_BN = 256;
 constexpr int TMEM_COLS = 2 * MAX_BN;
-constexpr int kChain = 40;                       // stages between drains: 2,560 rows
+// Stages between drains: 2,560 rows of bf16, 1,152 of fp16, whose longer products lose more to the tensor cores' truncation.  Off by, against 64 bits,
+// 22,725 x 200 x 671 fp16: 1.3e-6 with 40 stages, 8e-7 with 18 (sums rounded to nearest: 2e-7); bf16 with 40: 5e-7.  475,136 x 1,024 x 256 fp16 takes 288 us
+// instead of 261 for it.
+constexpr int kChain = 40, kChainF16 = 18;
+template <typename TG>
+__host__ __device__ constexpr int chain_of() { return top_binade<TG>() == 15 ? kChainF16 : kChain; }
 // An item's first chain: of another length for neighbouring items, so that the CTAs do not all drain at once (they add into L2 at its rate
 // for atomics, 4.8 TB/s, and the MMAs of two accumulators wait)
-__device__ __forceinline__ int first_chain(int item) { return kChain - (item % 8) * (kChain / 8); }
+template <typename TG>
+__device__ __forceinline__ int first_chain(int item) { return chain_of<TG>() - (item % 8) * chain_of<TG>() / 8; }
 
 // CTAS: 1, or 2: a pair.  MH: accumulators of 128 columns of g beside each other per CTA.
 template <int CTAS, int MH>
@@ -99,7 +105,7 @@ __device__ __forceinline__ Item item_of(int w, const Args& p) {
   return it;
 }
 
-// With one k tile g is read once and should not displace the partial tiles from the L2 (475,136 x 1,024 x 256 265 -> 259 us, back to back 325 -> 316;
+// With one k tile g is read once and should not displace the partial tiles from the L2 (475,136 x 1,024 x 256, chains of 2,560 rows, 265 -> 259 us, back to back 325 -> 316;
 // with more of them each reads g, and the hint costs 8 %)
 __device__ __forceinline__ uint64_t evict_first() {
   uint64_t policy;
@@ -272,7 +278,7 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
           if (!mbar_wait<PAIR>(smem_u32(&sh->acc_empty[buf]), acc_phase, abort)) { give_up(sh, status, 3); ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem_base + buf * MAX_BN;
-          n = min(left, n == 0 ? first_chain(w) : kChain);
+          n = min(left, n == 0 ? first_chain<TG>(w) : chain_of<TG>());
           for (int i = 0; i < n; ++i) {
             // the converters' arrivals stand for g too
             if (!mbar_wait<PAIR>(smem_u32(&sh->full_x[slot]), phase, abort)) { give_up(sh, status, 4); ok = false; break; }
@@ -384,7 +390,7 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
     for (int w = w_first; w < n_items && ok; w += w_step) {
       const Item m = item_of(w, p);
       float* part = p.parts + (((int64_t)(m.nt * p.k_tiles + m.kt) * p.splits + m.split) * (4 * CTAS * MH) + (rank * MH + half) * 4 + quad) * (p.bn * 32) + lane * 4;
-      for (int kb = m.kb0; kb < m.kb1; kb += kb == m.kb0 ? first_chain(w) : kChain, ++chains) {
+      for (int kb = m.kb0; kb < m.kb1; kb += kb == m.kb0 ? first_chain<TG>(w) : chain_of<TG>(), ++chains) {
         const int buf = F::BUFS == 2 ? chains & 1 : 0;
         if (!mbar_wait_warp(smem_u32(&sh->acc_full[buf]), (F::BUFS == 2 ? chains >> 1 : chains) & 1, abort)) {
           if (lane == 0) give_up(sh, status, 8);
