@@ -229,10 +229,11 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_g, Args p, int* status) {
   tc_fence_after();
   const uint32_t tmem_base = sh->tmem_base;
   pdl_begin();
-  // an arrival at the leader's barrier
+  // an arrival at the leader's barrier; its MMA issuer waits for it at cluster scope
   auto arrive_leader = [&](uint64_t* bar) {
-    if (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(bar), 0));
-    else mbar_arrive(smem_u32(bar));
+    const uint32_t at = PAIR ? map_to_cta(smem_u32(bar), 0) : smem_u32(bar);
+    if (PAIR) mbar_arrive_cluster(at);
+    else mbar_arrive(at);
   };
 
   if (warp == 0) {

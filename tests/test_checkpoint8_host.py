@@ -127,3 +127,17 @@ def test_python_refusals(native):
             c8.Checkpoint8(**a)
     with pytest.raises(TypeError):
         c8.Checkpoint8(codes, exps, "int8", (4, 32), torch.float64)
+
+
+def test_weight_gradient_barriers_of_both_ctas_are_awaited_at_cluster_scope():
+    """Barriers that the other CTA of a pair arrives at are waited for with an acquire of cluster scope, and groups that wait by
+    parity divide the ring's stages."""
+    import re
+    from pathlib import Path
+    text = (Path(__file__).resolve().parent.parent / "beatsaberrl_b200" / "csrc" / "wgrad8_tc5.cu").read_text()
+    arrived = set(re.findall(r"arrive_leader\(&sh->(\w+)", text))
+    assert arrived == {"full_x", "acc_empty"} and text.count("mbar_arrive_cluster(") == 1
+    for bar in arrived:
+        calls = re.findall(r"(mbar_wait\w*)(<[^>]*>)?\(smem_u32\(&sh->" + bar + r"\[", text)
+        assert calls and all(scope == "<PAIR>" for _, scope in calls), (bar, calls)
+    assert "static_assert(STAGES % GROUPS == 0 && STAGES % SUM_GROUPS == 0" in text
