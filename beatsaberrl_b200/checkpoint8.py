@@ -144,6 +144,10 @@ class Checkpoint8:
         self._exps_ptr = self._codes_ptr + rows * blocks * BLOCK
         return self
 
+    def __reduce__(self):
+        """Copies and pickles are made anew from codes and exps, with the constructor's checks: the addresses kept here are this one's own."""
+        return Checkpoint8, (self.codes, self.exps, self.kind, self.shape, self.dtype)
+
     @property
     def codes(self) -> torch.Tensor:
         m = self._memory

@@ -641,3 +641,29 @@ def test_linear_of_slices(c8):
         assert ((results[0][0].double() - (x @ w.t() + b)).abs() <= half_step(x @ w.t() + b, F16) + most * (k + 2) * U).all()
         want = gy @ w
         assert ((results[0][1].double() - want).abs() <= half_step(want, F16) + (gy.abs() @ w.abs()) * (n + 2) * U).all()
+
+
+def test_copies_have_their_own_memory(c8):
+    """deepcopy and pickle: the copy outlives the original; one that lands on the CPU is refused."""
+    import copy
+    import io
+    import pickle
+    x = randn(5, 3, 70, g=gen(29), dtype=F16)
+    for kind in ("int8", "e4m3"):
+        one = c8.pack8(x, kind)
+        want, bits = one.expand(), one.codes.clone()
+        for kept in (one, c8.Checkpoint8(one.codes.clone(), one.exps.clone(), kind, x.shape, F16)):
+            stored = io.BytesIO()
+            torch.save(kept, stored)
+            copies = [copy.deepcopy(kept), pickle.loads(pickle.dumps(kept)), torch.load(io.BytesIO(stored.getvalue()), weights_only=False)]
+            same = copy.copy(kept)
+            assert torch.equal(same.expand(), want)
+            kept.codes.zero_()
+            assert not same.expand().any()
+            for c in copies:
+                assert c.shape == x.shape and c.dtype == F16 and c.kind == kind and torch.equal(c.expand(), want) and torch.equal(c.codes, bits)
+                own = {c.codes.data_ptr(), kept.codes.data_ptr()}
+                assert len(own) == 2 and c._codes_ptr == c.codes.data_ptr() and c._exps_ptr == c.exps.data_ptr()
+            with pytest.raises(RuntimeError, match="CUDA"):
+                torch.load(io.BytesIO(stored.getvalue()), weights_only=False, map_location="cpu")
+
