@@ -156,6 +156,7 @@ _sig = {
     "bsrl_layernorm8_bwd": (C.c_int, [_P, C.c_int32, C.c_int64, _P, C.c_int64, _P, _P, C.c_int32, _P, _P, _P, C.c_int64, C.c_int32, _P,
                                       C.c_int32, C.c_int64, _P, _P, _P, C.c_int64, _P]),
     "bsrl_linear8_wgrad_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    "bsrl_linear8_wgrad_plan": (C.c_int, [C.c_int64, C.c_int32, C.c_int32, C.POINTER(C.c_int32)]),
     "bsrl_linear8_wgrad": (C.c_int, [_P, C.c_int32, C.c_int64, _P, _P, C.c_int32, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, C.c_int64,
                                      _P]),
     "bsrl_attention_tokens": (C.c_int, [_P, _P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P]),

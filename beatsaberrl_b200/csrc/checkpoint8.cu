@@ -147,6 +147,17 @@ int64_t bsrl_linear8_wgrad_workspace_bytes(int64_t rows, int32_t n, int32_t k, i
   return rows == 0 ? 0 : wgrad8_workspace(rows, n, k, aligned != 0);
 }
 
+int bsrl_linear8_wgrad_plan(int64_t rows, int32_t n, int32_t k, int32_t* plan) {
+  const char* me = "linear8_wgrad_plan";
+  if (rows < 1 || rows > 0x7fffff00 - 1 || n < 1 || k < 1 || n > kMaxSide || k > kMaxSide || (int64_t)n * k > kMaxWeight)
+    return refuse(BSRL_ERR_SHAPE, me, "rows must be 1 .. 2^31 - 257, n and k 1 .. 2^20, n k at most 2^31");
+  if (!plan) return refuse(BSRL_ERR_NULL, me, "NULL plan");
+  int32_t p[3];
+  wgrad8_plan(rows, n, k, p);
+  for (int i = 0; i < 3; ++i) plan[i] = p[i];
+  return BSRL_OK;
+}
+
 int bsrl_linear8_wgrad(const void* gy, int32_t gy_dtype, int64_t ldgy, const uint8_t* codes, const uint8_t* exps, int32_t kind, int64_t rows,
                        int32_t n, int32_t k, float* g_weight, float* g_bias, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* me = "linear8_wgrad";

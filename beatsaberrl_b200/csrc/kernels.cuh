@@ -409,6 +409,7 @@ int norm8_bwd(const Norm8BwdArgs& a, float* workspace, cudaStream_t stream);
 // Weight and bias gradient of a linear layer from its input in 8 bits (wgrad8_tc5.cu); gb may be nullptr.  aligned: g and its pitch
 // are multiples of 16 bytes.
 int64_t wgrad8_workspace(int64_t rows, int n, int k, bool aligned);
+void wgrad8_plan(int64_t rows, int n, int k, int32_t (&plan)[3]);      // columns of g and of x per tile, pieces of the rows
 int wgrad8(const void* g, int g_dtype, int64_t ldg, const uint8_t* codes, const uint8_t* exps, int kind, int64_t rows, int n, int k, float* gw,
            int64_t ldw, float* gb, void* workspace, int64_t workspace_bytes, cudaStream_t stream);
 

@@ -614,6 +614,13 @@ int64_t wgrad8_workspace(int64_t rows, int n, int k, bool aligned) {
   return pl.copy_bytes + pl.parts_bytes + pl.bias_bytes;
 }
 
+void wgrad8_plan(int64_t rows, int n, int k, int32_t (&plan)[3]) {
+  const Plan pl = plan_of(rows, n, k, false);
+  plan[0] = pl.tile_n();
+  plan[1] = pl.bn;
+  plan[2] = pl.splits;
+}
+
 int wgrad8(const void* g, int g_dtype, int64_t ldg, const uint8_t* codes, const uint8_t* exps, int kind, int64_t rows, int n, int k, float* gw,
            int64_t ldw, float* gb, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
   const Plan pl = plan_of(rows, n, k, needs_copy(g, ldg));

@@ -337,8 +337,11 @@ int bsrl_layernorm8_bwd(const void* gy, int32_t gy_dtype, int64_t ldgy, const vo
  * gy's type.  rows up to 2^31 - 257, n and k up to 2^20, n k up to
  * 2^31.  Make the first call on a device outside any stream capture.  workspace: bsrl_linear8_wgrad_workspace_bytes() of device
  * memory, 256-byte aligned; `aligned` says that gy starts on 16 bytes and ldgy is a multiple of 8 (else the workspace also takes
- * a copy of gy that is). */
+ * a copy of gy that is).  bsrl_linear8_wgrad_plan: how the current device's calls of this size are cut up, for tests and timings: plan[0] columns of
+ * gy per tile (128: one CTA each; 256: a pair of CTAs; 512: a pair with two accumulators per CTA), plan[1] columns of x per
+ * tile, plan[2] pieces of the rows, whose partial tiles are added up. */
 int64_t bsrl_linear8_wgrad_workspace_bytes(int64_t rows, int32_t n, int32_t k, int32_t aligned);
+int bsrl_linear8_wgrad_plan(int64_t rows, int32_t n, int32_t k, int32_t plan[3]);
 int bsrl_linear8_wgrad(const void* gy, int32_t gy_dtype, int64_t ldgy, const uint8_t* codes, const uint8_t* exps,
                        int32_t kind, int64_t rows, int32_t n, int32_t k, float* g_weight, float* g_bias, void* workspace,
                        int64_t workspace_bytes, void* stream);

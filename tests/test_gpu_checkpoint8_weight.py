@@ -1,0 +1,68 @@
+"""The weight gradient from inputs kept in 8 bits: every form of its kernel, by what the plan of a size says, against 64 bits.
+
+Tolerances: the tensor cores add 16 rows at a time and cut the sum off (2 U of what is added up); chains of at most 2,560 rows (fp16: 1,152) are
+added rounded to nearest (U each), and so are the pieces of the rows."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+U = 2.0 ** -24
+CHAIN = {F16: 1152, BF16: 2560}
+
+# rows, n, k -> columns of gy per tile on 148 SMs: one CTA, a pair, a pair with two accumulators per CTA.  Remainders of the last
+# stage (64 rows), of n and of k; one tile and several
+FORMS = [((70001, 64, 64), 128), ((9000, 384, 640), 128), ((20000, 256, 256), 256), ((22725, 200, 671), 256), ((33646, 1985, 10), 512),
+         ((20994, 1916, 432), 512), ((49844, 1197, 690), 512)]
+
+
+@pytest.fixture(scope="module")
+def c8(native):
+    from beatsaberrl_b200 import checkpoint8
+    return checkpoint8
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out(native):
+    yield
+    native.check(native.lib.bsrl_device_status())
+
+
+def plan_of(native, rows, n, k):
+    """(columns of gy per tile, columns of x per tile, 64-row stages of a piece of the rows)"""
+    p = (C.c_int32 * 3)()
+    native.check(native.lib.bsrl_linear8_wgrad_plan(rows, n, k, p))
+    return p[0], p[1], math.ceil(rows / 64) // p[2]
+
+
+def operands(c8, rows, n, k, dtype, kind):
+    g = torch.Generator(device="cuda").manual_seed(rows + n + k)
+    kept = c8.pack8(torch.randn(rows, k, generator=g, device="cuda").to(dtype), kind)
+    return torch.randn(rows, n, generator=g, device="cuda").to(dtype), kept
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("shape,tile_n", FORMS)
+def test_every_form(native, c8, shape, tile_n, dtype, kind):
+    rows, n, k = shape
+    form, _, stages = plan_of(native, rows, n, k)
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert form == tile_n
+    gy, kept = operands(c8, rows, n, k, dtype, kind)
+    gw, gb = c8.linear8_weight_grad(gy, kept)
+    x, g = kept.expand().double(), gy.double()
+    chains = math.ceil((stages + 1) * 64 / CHAIN[dtype]) + 1        # the first one of a piece is shorter
+    pieces = math.ceil(rows / 64 / stages)
+    most = g.abs().t() @ x.abs()
+    assert ((gw.double() - g.t() @ x).abs() <= most * (CHAIN[dtype] / 16 * 2 + chains + pieces) * U).all()
+    # a lane adds at most every fourth row of its piece, and there are at most 12 partial sums per piece
+    assert ((gb.double() - g.sum(0)).abs() <= g.abs().sum(0) * ((stages + 1) * 16 + 12 * pieces) * U).all()
+    again, none = c8.linear8_weight_grad(gy, kept, bias=False)
+    assert none is None and torch.equal(again, gw)
+    a, b = c8.linear8_weight_grad(torch.cat([gy[:, :1], gy], 1)[:, 1:], kept)       # rows that have to be copied
+    assert torch.equal(a, gw) and torch.equal(b, gb)
