@@ -66,3 +66,20 @@ def test_every_form(native, c8, shape, tile_n, dtype, kind):
     assert none is None and torch.equal(again, gw)
     a, b = c8.linear8_weight_grad(torch.cat([gy[:, :1], gy], 1)[:, 1:], kept)       # rows that have to be copied
     assert torch.equal(a, gw) and torch.equal(b, gb)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("shape", [(22725, 200, 671), (475136, 128, 128), (49844, 1197, 690), (475136, 1024, 256)])
+def test_long_pieces_stay_near_the_64_bit_sums(native, c8, shape, dtype, kind):
+    """What drains between chains are for.  A running sum S kept to 25 bits loses half of its last place per step on average, 0.36 x 2^-24 |S|
+    (a number's last place is 0.72 x 2^-24 of it on average), always towards zero.  Over a chain of M products of 16 rows of independent
+    numbers S grows with the square root of the rows, so that the losses add up to M / sqrt(3) times that of the chain's sum, and
+    as much in relation of the sum of many chains: 1.24e-8 M.  fp16, M = 72: 8.9e-7, and 2e-7 of sums rounded to nearest across it: 9.1e-7.  Chains of
+    26 stages (M = 104) are past the bound where a piece holds many.  bf16's products have fewer bits, of which less is cut off: its chains are longer, the bound is the same."""
+    rows, n, k = shape
+    assert plan_of(native, rows, n, k)[2] > 26                  # stages of a piece: well past the 18 of a chain of fp16
+    gy, kept = operands(c8, rows, n, k, dtype, kind)
+    want = gy.double().t() @ kept.expand().double()
+    gw, _ = c8.linear8_weight_grad(gy, kept)
+    assert float((gw.double() - want).norm() / want.norm()) < 1.05e-6
