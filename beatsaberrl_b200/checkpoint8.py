@@ -312,7 +312,11 @@ def layer_norm8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
 
 # ------------------------------------------------------------------ linear
 def linear8_weight_grad(gy: torch.Tensor, kept: Checkpoint8, bias: bool = True):
-    """(g_weight (n, k), g_bias (n) or None) in fp32 of y = x w^T + b, from gy (..., n) float16 or bfloat16 and x (..., k) in 8 bits."""
+    """(g_weight (n, k), g_bias (n) or None) in fp32 of y = x w^T + b, from gy (..., n) float16 or bfloat16 and x (..., k) in 8 bits.
+
+    x enters the product as ``kept.expand(gy.dtype)`` has it.  That is exact for a bfloat16 gy and for a float16 gy with a float16 activation down to
+    fp16's smallest step; a float16 gy takes what a float32 or bfloat16 activation holds past 65,504 as infinity, and below 2^-25 as
+    zero.  Such activations want a bfloat16 gy, or to be scaled ahead of ``pack8``."""
     if gy.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"gy must be float16 or bfloat16, got {gy.dtype}")
     if gy.shape[:-1] != kept.shape[:-1] or gy.device != kept.device:

@@ -337,7 +337,7 @@ int bsrl_layernorm8_bwd(const void* gy, int32_t gy_dtype, int64_t ldgy, const vo
 
 /* Weight and bias gradient of y = x w^T + b from x (rows, k) kept in 8 bits and gy (rows, n) f16 or bf16, on the tcgen05 tensor
  * cores: g_weight (n, k) = gy^T x8, g_bias (n) = column sums of gy (NULL: none); written, not added to.  x8 enters the product in
- * gy's type.  rows up to 2^31 - 257, n and k up to 2^20, n k up to
+ * gy's type, as bsrl_expand8 gives it: exact in bf16; in f16 infinity past 65,504 and zero below 2^-25, which a checkpoint of f32 or bf16 rows can hold.  rows up to 2^31 - 257, n and k up to 2^20, n k up to
  * 2^31.  Make the first call on a device outside any stream capture.  workspace: bsrl_linear8_wgrad_workspace_bytes() of device
  * memory, 256-byte aligned; `aligned` says that gy starts on 16 bytes and ldgy is a multiple of 8 (else the workspace also takes
  * a copy of gy that is).  bsrl_linear8_wgrad_plan: how the current device's calls of this size are cut up, for tests and timings: plan[0] columns of

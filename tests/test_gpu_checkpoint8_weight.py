@@ -83,3 +83,32 @@ def test_long_pieces_stay_near_the_64_bit_sums(native, c8, shape, dtype, kind):
     want = gy.double().t() @ kept.expand().double()
     gw, _ = c8.linear8_weight_grad(gy, kept)
     assert float((gw.double() - want).norm() / want.norm()) < 1.05e-6
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("x_dtype", [torch.float32, F16, BF16])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_activations_of_another_type(c8, dtype, x_dtype, kind):
+    """The product is that of the checkpoint expanded to the gradient's type: exact in range; an fp16 gradient takes what lies past fp16 as infinity, in
+    its own column only, and what lies below its smallest step as zero."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    rows, n, k = 300, 40, 96
+    x, gy = torch.randn(rows, k, generator=g, device="cuda"), torch.randn(rows, n, generator=g, device="cuda").to(dtype)
+    wide = x_dtype != F16
+    if wide:
+        x[7, 3] = 1e5                                   # past fp16; its neighbours in the block lose all but a step of 512 or 2
+        x[:, 32:64] = 1e-9                              # below fp16's smallest step
+    kept = c8.pack8(x.to(x_dtype), kind)
+    gw, gb = c8.linear8_weight_grad(gy, kept)
+    xv = kept.expand(dtype)
+    if dtype == BF16:
+        assert torch.equal(xv.double(), kept.expand(torch.float32).double())
+    bad = torch.isinf(xv).any(0)
+    assert bad.nonzero().flatten().tolist() == ([3] if wide and dtype == F16 else [])
+    assert (gw[:, bad].isfinite() == 0).all() and gw[:, ~bad].isfinite().all()
+    if wide:
+        assert (gw[:, 32:64] == 0).all() == (dtype == F16)
+    a, b = gy.double().t(), torch.where(bad, 0.0, xv.double())
+    # truncated once per 16 rows (2 U), then at most one sum per 64-row stage and piece
+    assert ((gw.double() - a @ b).abs()[:, ~bad] <= ((a.abs() @ b.abs()) * (rows / 16 * 2 + rows / 64 + 8) * U)[:, ~bad]).all()
+    assert ((gb.double() - gy.double().sum(0)).abs() <= gy.double().abs().sum(0) * rows * U).all()
