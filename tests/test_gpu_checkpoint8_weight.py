@@ -112,3 +112,33 @@ def test_activations_of_another_type(c8, dtype, x_dtype, kind):
     # truncated once per 16 rows (2 U), then at most one sum per 64-row stage and piece
     assert ((gw.double() - a @ b).abs()[:, ~bad] <= ((a.abs() @ b.abs()) * (rows / 16 * 2 + rows / 64 + 8) * U)[:, ~bad]).all()
     assert ((gb.double() - gy.double().sum(0)).abs() <= gy.double().abs().sum(0) * rows * U).all()
+
+
+def test_large_forms_at_once_and_replayed(c8):
+    """Calls of the form with two accumulators on two streams at the same time, and between a captured call's replays: none disturbs another."""
+    shapes = [(33646, 1985, 10), (20994, 1916, 432)]
+    ins = [operands(c8, *s, F16, "int8") for s in shapes]
+    want = [c8.linear8_weight_grad(*i) for i in ins]
+    streams = [torch.cuda.Stream() for _ in ins]
+    outs = [None, None]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[j] = c8.linear8_weight_grad(*ins[j])
+    torch.cuda.synchronize()
+    for out, w in zip(outs, want):
+        assert all(torch.equal(p, q) for p, q in zip(out, w))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        held = c8.linear8_weight_grad(*ins[1])
+    for _ in range(3):
+        graph.replay()
+        other = c8.linear8_weight_grad(*ins[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, want[1])) and all(torch.equal(p, q) for p, q in zip(other, want[0]))
+    for t in ins[1]:
+        (t if torch.is_tensor(t) else t.codes).zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not held[0].any() and not held[1].any()
