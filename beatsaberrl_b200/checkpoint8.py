@@ -1,7 +1,7 @@
 """Training operators that keep what their backward needs in 8 bits: LayerNorm, exact GELU and linear layers.
 
-A minibatch's saved activations bound its size.  These operators write an activation's 8-bit form (``Checkpoint8``) in the pass that reads
-it anyway, and their backward reads that form: 33/64 of the memory of 16-bit activations, 33/128 of fp32 ones.  Blocks of 32
+A minibatch's saved activations bound its size.  These operators write an activation's 8-bit form (``Checkpoint8``) -- LayerNorm and GELU in the
+pass that reads it anyway, ``linear8`` in one of its own; without grad mode too -- and their backward reads that form: 33/64 of the memory of 16-bit activations, 33/128 of fp32 ones.  Blocks of 32
 neighbouring values of a row share a power of two; ``kind`` "int8" is off by at most 1/127 of a block's largest magnitude, "e4m3" by
 2^-4 of every value.  ``include/bsrl.h`` ("activations kept in 8 bits") has the format, for reading it elsewhere.
 
@@ -234,8 +234,9 @@ def layer_norm8_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[to
     """LayerNorm over the last dimension of z = x + residual (rounded to x's type): (y, z, saved).
 
     weight and bias are fp32.  y has ``out_dtype`` (default: x's type): any of the three for fp32 rows, their own for 16-bit ones.
-    Without a residual z is x.  Rows are at most 8,192 wide.  What is kept is z: rows whose mean lies far beyond their spread keep little
-    of the spread."""
+    Without a residual z is x.  Rows are at most 8,192 wide and fastest where they start on 16 bytes (fp32 on
+    32, weight and bias too).  What is kept is z: rows whose mean lies far beyond their spread keep little of the spread, and where that is less than a
+    step of the 8 bits (equal values; a single one) the gradient is not small but wrong, by up to the square of (step / spread)."""
     code, k = _dtype(x, "x"), _kind(kind)
     m, rows, d, ld = _rows(x, "x")
     dev = x.device

@@ -140,7 +140,8 @@ constexpr int kResident = 2;
 // Threads of blocks that hold a row, per SM, and blocks of kThreads: what registers are kept free for.  Unaligned rows run more warps than
 // aligned ones and one row at a time: they wait for what follows from what a piece's place in memory is.  60,007 x 1,001 fp16 with a residual, 512 / 768
 // threads: forward 240 / 201 us, backward 214 / 179; 100,003 x 509, two / three blocks: forward 197 / 170.  Aligned forward, 14,848 x 8,192 fp32, 512 / 1,024
-// threads 191 / 162 us; its backward 231 / 245.
+// threads 191 / 162 us; its backward 231 / 245.  The unaligned backward above 4,096 columns, two steps per lane, pays for its 80 registers with about
+// 450 to 510 bytes of spills; above 6,144 columns its one block would fit 128 (not measured).
 constexpr int block_threads(int tpr, bool aligned, bool bwd) { return tpr > 0 ? kThreads : !aligned ? 768 : bwd ? 512 : 1024; }
 constexpr int blocks_per_sm(int tpr, bool aligned, bool bwd) { return tpr == 0 ? 1 : aligned || bwd ? kResident : 3; }
 
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(block_threads(TPR, ALIGNED, true), blocks_per_
 }
 
 // rows a team works on together (backward of 475,136 x 256: one 224 us, two 160, three 191, four 173; of 237,568 x 512: one 167, two 157; unaligned, of
-// 100,003 x 509: one 174, two 229)
+// 100,003 x 509: one 174, two 229).  All without a residual; with one, two rows of 257 to 512 spill 72 bytes (fp32 rows 216 to 268), not measured against one.
 constexpr int rows_together(int tpr, int nv, bool aligned, bool bwd) { return aligned && (bwd ? nv == 1 || tpr > 0 : nv == 1 && tpr > 0) ? 2 : 1; }
 
 // How rows of d elements are shared out: lanes per team (TPR), steps per lane, rows worked on together
@@ -500,7 +501,8 @@ struct Shape {
   int resident;            // blocks per SM
 };
 constexpr int kMaxWidth = 8192;
-// Rows above 512: by blocks (65,536 x 1,024 bf16 with a residual: forward 104 us, a warp's lanes with four pieces each 110; backward 113 / 202)
+// Rows above 512: by blocks (65,536 x 1,024 bf16 with a residual: forward 104 us, a warp's lanes with four pieces each 110; backward 113 / 202).  fp32 rows of
+// that width lose by it in the forward: 90 us, by a warp's lanes 84; the rule takes no note of the type.
 inline Shape shape_of(int d, bool aligned, bool bwd) {
   const int pieces = (int)pitch_of(d) / 8;
   Shape s;

@@ -37,9 +37,11 @@ constexpr int BK = 64;                           // rows per stage
 constexpr int BLOCK_BYTES = BK * 128;            // 64 columns x 64 rows of 16 bits
 constexpr int MAX_BN = 256;
 constexpr int TMEM_COLS = 2 * MAX_BN;
-// Stages between drains: 2,560 rows of bf16, 1,152 of fp16, whose longer products lose more to the tensor cores' truncation.  Off by, against 64 bits,
-// 22,725 x 200 x 671 fp16: 1.3e-6 with 40 stages, 8e-7 with 18 (sums rounded to nearest: 2e-7); bf16 with 40: 5e-7.  475,136 x 1,024 x 256 fp16 takes 288 us
-// instead of 261 for it.
+// Stages between drains: 2,560 rows of bf16, 1,152 of fp16, whose longer products lose more to the tensor cores' truncation.  Norm of the error against
+// 64 bits over that of the sums, normal numbers, int8 / e4m3: 22,725 x 200 x 671 fp16 1.2e-6 / 1.3e-6 with 40 stages, 7.1e-7 / 7.6e-7 with 18; in longer pieces 2.2e-6 and 9.1e-7;
+// bf16 with 40 up to 5.7e-7 / 7.9e-7.  bf16 gains by blocks that share an exponent from row to row: with rows whose sizes differ by a factor of e 1.6e-6 (fp16 1.3e-6), of
+// e^2 3.7e-6; with k = 1 1.5e-6 to 2e-6.  An fp32 product of 100,003 x 1,000 x 513: 1.9e-6 to 4.6e-6, rows by e^2 6.4e-6.  475,136 x 1,024 x 256 fp16 takes 288 us
+// instead of 261 for its chains.
 constexpr int kChain = 40, kChainF16 = 18;
 template <typename TG>
 __host__ __device__ constexpr int chain_of() { return top_binade<TG>() == 15 ? kChainF16 : kChain; }
@@ -566,7 +568,9 @@ Plan plan_of(int64_t rows, int n, int k, bool copy) {
       const int n_tiles = (n + 128 * ctas * mh - 1) / (128 * ctas * mh), units = sms / ctas;
       const int64_t tiles = (int64_t)n_tiles * k_tiles;
       if (tiles > 1 << 20) continue;
-      // cycles of a stage and of a drain that nothing hides (an item's last one; with one set of accumulators every one); bytes of partial tiles, all SMs
+      // cycles of a stage and of a drain that nothing hides (an item's last one; with one set of accumulators every one); bytes of partial tiles, all SMs.
+      // It ranks forms and splits and does not foretell times: 100,003 x 1,000 x 513 comes out at 77 us (measured 181), 475,136 x 1,024 x 256 at 150 (259 to 288).  Drains
+      // are counted by bf16's chains for either type, fewer than fp16 has; with fp16's 44 of 2,000 drawn sizes would take another form (not measured).
       const double stage = fmax((form == 0 ? 4.0 : form == 1 ? 3.1 : 4.6) * bn, form == 2 ? 700.0 : 450.0), drain = 2000 + 8.0 * mh * bn;
       // pieces of the rows: as fill one or more waves of SMs, or stages of some length each
       for (int i = 0; i < 10; ++i) {

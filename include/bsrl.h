@@ -293,8 +293,8 @@ int bsrl_linear_bwd(const void* g_f16, const void* x_f16, const void* w_f16, int
  * Values have at most 8 significant bits: bf16 holds them exactly, fp16 as far as its range goes.
  *
  * Matrices have elements of BSRL_F32, BSRL_F16 or BSRL_BF16, rows `ld` elements apart (ld >= d) and no alignment but
- * their elements'; rows that start on 16 bytes (f32: 32), with d a multiple of 8, are faster.  rows may be 0.  d up to 2^31 - 64
- * (bsrl_layernorm8: 8,192).  gamma, beta, mean, rstd and parameter gradients are fp32.  Sums are in fp32 and in one
+ * their elements'; rows that start on 16 bytes (f32: 32), with d a multiple of 8, are faster (bsrl_layernorm8: gamma and beta
+ * on 32 bytes too).  rows may be 0.  d up to 2^31 - 64 (bsrl_layernorm8: 8,192).  gamma, beta, mean, rstd and parameter gradients are fp32.  Sums are in fp32 and in one
  * order: a call on the same inputs gives the same bits.  Nothing may overlap except where said. */
 typedef enum bsrl_kind8 { BSRL_INT8 = 0, BSRL_E4M3 = 1 } bsrl_kind8;
 
@@ -322,8 +322,8 @@ int bsrl_gelu8_bwd(const void* gy, int32_t dtype, int64_t ldgy, const uint8_t* c
  * bsrl_layernorm8_bwd, with h = (z8 - mean) rstd and gh = gy gamma:
  *   gx = rstd (gh - mean(gh) - h mean(gh h)) (+ g_residual, the gradient that reaches z by other ways; may be NULL), in `dtype`
  *   g_gamma = sum over rows of gy h, g_beta = sum over rows of gy (written, not added to; either may be NULL)
- * The statistics are those of z itself, h is as near to the normalised z as the checkpoint to z in units of the row's spread: a row
- * that spreads by less than its blocks' step (a mean far beyond its variance; a single element) has little of a gradient left.
+ * The statistics are those of z itself, h is as near to the normalised z as the checkpoint to z in units of the row's spread: in a row
+ * that spreads by less than its blocks' step (a mean far beyond its variance; a single element) h is far above 1 and gx, which goes with its square, far too large.
  * gx is the gradient of x and of the residual.  gx may be g_residual, or gy where the types agree.  workspace:
  * bsrl_layernorm8_bwd_workspace_bytes() of device memory, 16-byte aligned (0 bytes: may be NULL). */
 int bsrl_layernorm8(const void* x, const void* residual, int32_t dtype, int64_t ldx, int64_t ldr, const float* gamma,
@@ -337,8 +337,8 @@ int bsrl_layernorm8_bwd(const void* gy, int32_t gy_dtype, int64_t ldgy, const vo
 
 /* Weight and bias gradient of y = x w^T + b from x (rows, k) kept in 8 bits and gy (rows, n) f16 or bf16, on the tcgen05 tensor
  * cores: g_weight (n, k) = gy^T x8, g_bias (n) = column sums of gy (NULL: none); written, not added to.  x8 enters the product in
- * gy's type, as bsrl_expand8 gives it: exact in bf16; in f16 infinity past 65,504 and zero below 2^-25, which a checkpoint of f32 or bf16 rows can hold.  rows up to 2^31 - 257, n and k up to 2^20, n k up to
- * 2^31.  Make the first call on a device outside any stream capture.  workspace: bsrl_linear8_wgrad_workspace_bytes() of device
+ * gy's type, as bsrl_expand8 gives it: exact in bf16; in f16 infinity past 65,504 and zero below 2^-25, which a checkpoint of f32 or bf16 rows
+ * can hold.  rows up to 2^31 - 257, n and k up to 2^20, n k up to 2^31.  Make the first call on a device outside any stream capture.  workspace: bsrl_linear8_wgrad_workspace_bytes() of device
  * memory, 256-byte aligned; `aligned` says that gy starts on 16 bytes and ldgy is a multiple of 8 (else the workspace also takes
  * a copy of gy that is).  bsrl_linear8_wgrad_plan: how the current device's calls of this size are cut up, for tests and timings: plan[0] columns of
  * gy per tile (128: one CTA each; 256: a pair of CTAs; 512: a pair with two accumulators per CTA), plan[1] columns of x per
