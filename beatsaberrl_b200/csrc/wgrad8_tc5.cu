@@ -570,7 +570,8 @@ Plan plan_of(int64_t rows, int n, int k, bool copy) {
       if (tiles > 1 << 20) continue;
       // cycles of a stage and of a drain that nothing hides (an item's last one; with one set of accumulators every one); bytes of partial tiles, all SMs.
       // It ranks forms and splits and does not foretell times: 100,003 x 1,000 x 513 comes out at 77 us (measured 181), 475,136 x 1,024 x 256 at 150 (259 to 288).  Drains
-      // are counted by bf16's chains for either type, fewer than fp16 has; with fp16's 44 of 2,000 drawn sizes would take another form (not measured).
+      // are counted by bf16's chains for either type, fewer than fp16 has: with fp16's own 44 of 2,000 drawn sizes take another form, and of 20 of those 5 were 2 to 13 % faster
+      // for it and 12 slower (73,077 x 280 x 1,711: 163 -> 290 us), since the stages' costs are off by more than the drains.
       const double stage = fmax((form == 0 ? 4.0 : form == 1 ? 3.1 : 4.6) * bn, form == 2 ? 700.0 : 450.0), drain = 2000 + 8.0 * mh * bn;
       // pieces of the rows: as fill one or more waves of SMs, or stages of some length each
       for (int i = 0; i < 10; ++i) {
